@@ -300,7 +300,8 @@ rg_status rg_linear_i8_noalloc(const float* x, int64_t m, int64_t k, const int8_
 /* The status a run reports for its device error words (no counterpart in the
  * reference): words[0] set -> RG_ERR_TIMEOUT (a tensor-core kernel gave up on a
  * bounded wait), words[1] set -> RG_ERR_INVALID_ARG (an embedding id not below
- * the vocabulary size), else RG_OK.  Host-only; every run and kernel-level call
+ * the vocabulary size; an index or length of a serving call out of its range),
+ * else RG_OK.  Host-only; every run and kernel-level call
  * maps its words through it. */
 rg_status rg_status_from_error_words(const int32_t words[2]);
 /* Test hook of the bounded-wait failure path (no counterpart in the reference):
@@ -334,6 +335,123 @@ rg_status rg_attention_f32(const float* qkv, int64_t ld, int64_t batch, int32_t 
  * common-range tanh (and GELU through it) against the general one, on every
  * input where the epilogue uses it.  Synchronous, current device, ~0.3 s. */
 rg_status rg_selftest_fast_paths(uint64_t mismatches[6]);
+
+/* ---------------------------------------------------------------------------
+ * Decoder serving (extensions; the reference has no key/value cache, no rotary
+ * positions and one activation scale per batch).  Device pointers, enqueued on
+ * `stream` of the current device; the calls never wait, allocate or copy to the
+ * host, so they can be captured.  What only the device can see (a bounded wait
+ * that gave up, a position, slot, page or length out of its range) is reported
+ * through `error_words`: two zeroed int32 words of device memory that any number
+ * of calls may share; a call only ever sets them, and
+ * rg_status_from_error_words maps a host copy to a status.  What an out-of-range
+ * index names is never accessed: the token, page or sequence is skipped (its
+ * output is not written, or a page's keys count as zeros).
+ * A call of zero rows, tokens or sequences returns RG_OK and launches nothing.
+ * ------------------------------------------------------------------------- */
+typedef enum rg_dtype { RG_DTYPE_F32 = 0, RG_DTYPE_F16 = 1, RG_DTYPE_BF16 = 2 } rg_dtype;
+
+/* One scale per row (token): x [rows, k] (row stride ldx elements) -> q [rows, ldq] i8
+ * (columns k..ldq zero, ldq a multiple of 16), scale[r] = absmax of the row (NaN ignored)
+ * < 1e-12 ? 1 : absmax / 127, each value QuantTensor::from_f32's
+ * (src/inference/quantize.rs:18-35) with the row's scale. */
+rg_status rg_quantize_token_i8(const void* x, int32_t x_dtype, int64_t rows, int64_t k, int64_t ldx, int8_t* q,
+                               int64_t ldq, float* scale, void* stream);
+/* out[r, c] = act(f32(sum_k a[r,k] * w[c,k]) * (a_scale[r] * w_scale[c]) + bias[c]), rounded
+ * once to out_dtype: int8_gemm_fused with one scale per token and one per output channel.
+ * a [m, ld], w [n, ld] i8 as for rg_gemm_i8_fused; bias may be NULL (0); out has row
+ * stride ldo elements. */
+rg_status rg_gemm_i8_token(const int8_t* a, const float* a_scale, const int8_t* w, const float* w_scale, int64_t m,
+                           int64_t n, int64_t ld, const float* bias, int32_t act, float act_param, void* out,
+                           int32_t out_dtype, int64_t ldo, int32_t* error_words, void* stream);
+/* The two in one call: x [m, k] (row stride ldx) against w [n, ld], ld >= k.  `workspace`
+ * holds rg_linear_i8_token_workspace_size(m, ld) bytes, 256-byte aligned, and is free
+ * again once the call's work on `stream` is done. */
+int64_t rg_linear_i8_token_workspace_size(int64_t m, int64_t ld);
+rg_status rg_linear_i8_token(const void* x, int32_t x_dtype, int64_t m, int64_t k, int64_t ldx, const int8_t* w,
+                             const float* w_scale, int64_t n, int64_t ld, const float* bias, int32_t act,
+                             float act_param, void* out, int32_t out_dtype, int64_t ldo, void* workspace,
+                             int32_t* error_words, void* stream);
+
+/* Rotary positions.  A table has one f32 row per position: rot_dim / 2 cosines, then
+ * rot_dim / 2 sines, of position * freq[i].  With freq[i] = base^(-2 i / rot_dim):
+ *   RG_ROPE_PLAIN   freq[i];
+ *   RG_ROPE_LINEAR  freq[i] / factor (positions interpolated);
+ *   RG_ROPE_BANDS   dimensions that turn at least fast_turns times within old_context
+ *                   positions keep freq[i], those that turn at most slow_turns times get
+ *                   freq[i] / factor, a linear ramp over the dimension index in between.
+ * Cosines and sines are multiplied by gain.  Angles are computed in 64 bits, so that
+ * far positions keep their phase; the result is rounded once to f32. */
+typedef enum rg_rope_kind { RG_ROPE_PLAIN = 0, RG_ROPE_LINEAR = 1, RG_ROPE_BANDS = 2 } rg_rope_kind;
+typedef struct rg_rope_scaling {
+  int32_t kind;
+  double base, factor, gain;
+  double old_context, fast_turns, slow_turns;
+} rg_rope_scaling;
+rg_status rg_rope_table_f32(const rg_rope_scaling* scaling, int64_t positions, int32_t rot_dim, float* table,
+                            void* stream);
+/* Rotates the first rot_dim dimensions of every head (rot_dim = the table's row length,
+ * even, <= head_dim) and copies the rest: for pair i of cosine c and sine s,
+ * (a, b) -> (a c - b s, b c + a s), with a, b dimensions i and i + rot_dim / 2, or 2 i and
+ * 2 i + 1 when `interleaved`.  x, out: [tokens, heads, head_dim], head_dim contiguous, the
+ * other strides in elements; out may be x (with the same strides).  Sums in f32. */
+rg_status rg_rope(const void* x, int32_t dtype, int64_t tokens, int32_t heads, int32_t head_dim,
+                  int64_t token_stride, int64_t head_stride, const int32_t* positions, const float* table,
+                  int64_t table_rows, int32_t rot_dim, int32_t interleaved, void* out, int64_t out_token_stride,
+                  int64_t out_head_stride, int32_t* error_words, void* stream);
+
+/* One layer's paged cache: `pages` pages of page_size tokens, keys and values in two
+ * tensors with the same strides (elements), head_dim contiguous; dtype f16 or bf16. */
+typedef struct rg_kv_cache {
+  void* k; void* v;
+  int32_t dtype, page_size, kv_heads, head_dim;
+  int64_t pages, page_stride, token_stride, head_stride;
+} rg_kv_cache;
+/* Appends k and v [tokens, kv_heads, head_dim] to the cache, k rotated on the way: token t
+ * goes to token slots[t] % page_size of page slots[t] / page_size; a negative slot is
+ * padding (nothing is stored).  Two tokens of one call must not share a slot.  With q
+ * [tokens, heads, head_dim] not NULL, q_out receives q rotated, in the cache's dtype.
+ * x_dtype (of q, k and v) is the cache's dtype or f32.  table NULL: nothing is rotated and
+ * positions may be NULL. */
+typedef struct rg_kv_append_args {
+  const void* k; const void* v; const void* q;
+  void* q_out;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+  const int64_t* slots;
+  const int32_t* positions;
+  const float* table;
+  int64_t table_rows, tokens;
+  int32_t x_dtype, heads, rot_dim, interleaved;
+} rg_kv_append_args;
+rg_status rg_kv_append(const rg_kv_cache* cache, const rg_kv_append_args* args, int32_t* error_words, void* stream);
+
+/* Attention of a chunk of new tokens over the cache.  Sequence b has the query tokens
+ * cu_q[b] .. cu_q[b + 1] - 1 of q [tokens, heads, head_dim] and kv_len[b] keys, the j-th in
+ * token j % page_size of page block_table[b, j / page_size] (entries past the last key are
+ * not read).  Its queries are the last of its tokens: with `causal`, query i sees keys
+ * j <= kv_len - q_len + i, else all of them.  heads is a multiple of kv_heads; query head h
+ * reads key head h / (heads / kv_heads).  out = softmax(scale * q k^T) v, a row that sees no
+ * key being zeros.  q and out have the cache's dtype; scores, the softmax's maximum and sum,
+ * and the output sum are f32; a probability is rounded to the cache's dtype before it
+ * multiplies v.  max_q_len and max_kv_len bound the lengths (they size the launch); a
+ * sequence whose lengths are out of range is reported and skipped.  head_dim: 64, 96, 128 or
+ * 256.  `workspace`: rg_attention_paged_workspace_size bytes, 256-byte aligned (NULL when
+ * that is 0), free again once the call's work on `stream` is done. */
+typedef struct rg_paged_attention_args {
+  const void* q; void* out;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* kv_len;
+  const int32_t* cu_q;
+  int64_t tokens;
+  int32_t batch, heads, max_q_len, max_kv_len, max_pages, causal;
+  float scale;
+} rg_paged_attention_args;
+int64_t rg_attention_paged_workspace_size(const rg_kv_cache* cache, const rg_paged_attention_args* args);
+rg_status rg_attention_paged(const rg_kv_cache* cache, const rg_paged_attention_args* args, void* workspace,
+                             int32_t* error_words, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Deterministic generator used by the benchmark configurations: SplitMix64

@@ -11,6 +11,9 @@
 
 use std::os::raw::{c_char, c_void};
 
+/// C's `double`.
+pub type double = f64;
+
 /// `rg_status`: every entry point returns one (0 = success).
 pub type rg_status = i32;
 pub const RG_OK: rg_status = 0;
@@ -68,6 +71,14 @@ pub const RG_TRACE_SCALES: i32 = 0;
 pub const RG_TRACE_AQ: i32 = 1;
 pub const RG_TRACE_ACC: i32 = 2;
 pub const RG_TRACE_OUT: i32 = 3;
+
+/// `rg_dtype` and `rg_rope_kind` of the decoder-serving entry points.
+pub const RG_DTYPE_F32: i32 = 0;
+pub const RG_DTYPE_F16: i32 = 1;
+pub const RG_DTYPE_BF16: i32 = 2;
+pub const RG_ROPE_PLAIN: i32 = 0;
+pub const RG_ROPE_LINEAR: i32 = 1;
+pub const RG_ROPE_BANDS: i32 = 2;
 
 pub const RG_LINEAR_NOALLOC_MAX_BYTES: u32 = 16 << 20;
 
@@ -157,6 +168,86 @@ pub struct rg_rng {
     pub state: u64,
 }
 
+/// How a rotary table's frequencies are scaled.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rg_rope_scaling {
+    pub kind: i32,
+    pub base: double,
+    pub factor: double,
+    pub gain: double,
+    pub old_context: double,
+    pub fast_turns: double,
+    pub slow_turns: double,
+}
+
+/// One layer's paged key / value cache.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rg_kv_cache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub dtype: i32,
+    pub page_size: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub pages: i64,
+    pub page_stride: i64,
+    pub token_stride: i64,
+    pub head_stride: i64,
+}
+
+/// New keys and values (and optionally queries) of `rg_kv_append`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rg_kv_append_args {
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub q: *const c_void,
+    pub q_out: *mut c_void,
+    pub k_token_stride: i64,
+    pub k_head_stride: i64,
+    pub v_token_stride: i64,
+    pub v_head_stride: i64,
+    pub q_token_stride: i64,
+    pub q_head_stride: i64,
+    pub q_out_token_stride: i64,
+    pub q_out_head_stride: i64,
+    pub slots: *const i64,
+    pub positions: *const i32,
+    pub table: *const f32,
+    pub table_rows: i64,
+    pub tokens: i64,
+    pub x_dtype: i32,
+    pub heads: i32,
+    pub rot_dim: i32,
+    pub interleaved: i32,
+}
+
+/// One call of `rg_attention_paged`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rg_paged_attention_args {
+    pub q: *const c_void,
+    pub out: *mut c_void,
+    pub q_token_stride: i64,
+    pub q_head_stride: i64,
+    pub out_token_stride: i64,
+    pub out_head_stride: i64,
+    pub block_table: *const i32,
+    pub block_table_stride: i64,
+    pub kv_len: *const i32,
+    pub cu_q: *const i32,
+    pub tokens: i64,
+    pub batch: i32,
+    pub heads: i32,
+    pub max_q_len: i32,
+    pub max_kv_len: i32,
+    pub max_pages: i32,
+    pub causal: i32,
+    pub scale: f32,
+}
+
 #[link(name = "rg_npu")]
 extern "C" {
     pub fn rg_last_error() -> *const c_char;
@@ -219,6 +310,30 @@ extern "C" {
     pub fn rg_attention_f32(qkv: *const f32, ld: i64, batch: i64, t: i32, heads: i32, head_dim: i32,
                             out: *mut f32, ldo: i64, stream: *mut c_void) -> rg_status;
     pub fn rg_selftest_fast_paths(mismatches: *mut u64) -> rg_status;
+
+    pub fn rg_quantize_token_i8(x: *const c_void, x_dtype: i32, rows: i64, k: i64, ldx: i64, q: *mut i8,
+                                ldq: i64, scale: *mut f32, stream: *mut c_void) -> rg_status;
+    pub fn rg_gemm_i8_token(a: *const i8, a_scale: *const f32, w: *const i8, w_scale: *const f32, m: i64,
+                            n: i64, ld: i64, bias: *const f32, act: i32, act_param: f32, out: *mut c_void,
+                            out_dtype: i32, ldo: i64, error_words: *mut i32, stream: *mut c_void) -> rg_status;
+    pub fn rg_linear_i8_token_workspace_size(m: i64, ld: i64) -> i64;
+    pub fn rg_linear_i8_token(x: *const c_void, x_dtype: i32, m: i64, k: i64, ldx: i64, w: *const i8,
+                              w_scale: *const f32, n: i64, ld: i64, bias: *const f32, act: i32,
+                              act_param: f32, out: *mut c_void, out_dtype: i32, ldo: i64,
+                              workspace: *mut c_void, error_words: *mut i32, stream: *mut c_void) -> rg_status;
+    pub fn rg_rope_table_f32(scaling: *const rg_rope_scaling, positions: i64, rot_dim: i32, table: *mut f32,
+                             stream: *mut c_void) -> rg_status;
+    pub fn rg_rope(x: *const c_void, dtype: i32, tokens: i64, heads: i32, head_dim: i32, token_stride: i64,
+                   head_stride: i64, positions: *const i32, table: *const f32, table_rows: i64, rot_dim: i32,
+                   interleaved: i32, out: *mut c_void, out_token_stride: i64, out_head_stride: i64,
+                   error_words: *mut i32, stream: *mut c_void) -> rg_status;
+    pub fn rg_kv_append(cache: *const rg_kv_cache, args: *const rg_kv_append_args, error_words: *mut i32,
+                        stream: *mut c_void) -> rg_status;
+    pub fn rg_attention_paged_workspace_size(cache: *const rg_kv_cache,
+                                             args: *const rg_paged_attention_args) -> i64;
+    pub fn rg_attention_paged(cache: *const rg_kv_cache, args: *const rg_paged_attention_args,
+                              workspace: *mut c_void, error_words: *mut i32,
+                              stream: *mut c_void) -> rg_status;
 
     pub fn rg_rng_seed(r: *mut rg_rng, seed: u64);
     pub fn rg_rng_next_u64(r: *mut rg_rng) -> u64;

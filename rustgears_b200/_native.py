@@ -18,6 +18,8 @@ RG_ERR_UNSUPPORTED, RG_ERR_IO, RG_ERR_OOM, RG_ERR_NO_DEVICE, RG_ERR_NO_PROFILE =
 RG_TRACE_SCALES, RG_TRACE_AQ, RG_TRACE_ACC, RG_TRACE_OUT = 0, 1, 2, 3
 RG_SESSION_NO_PROFILE, RG_SESSION_NO_FUSION, RG_SESSION_NO_GRAPH = 1, 2, 4
 RG_RUN_ASYNC = 1
+RG_DTYPE_F32, RG_DTYPE_F16, RG_DTYPE_BF16 = 0, 1, 2
+RG_ROPE_PLAIN, RG_ROPE_LINEAR, RG_ROPE_BANDS = 0, 1, 2
 
 
 class RgError(RuntimeError):
@@ -71,6 +73,37 @@ class RngC(C.Structure):
     _fields_ = [("state", C.c_uint64)]
 
 
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("base", C.c_double), ("factor", C.c_double), ("gain", C.c_double),
+                ("old_context", C.c_double), ("fast_turns", C.c_double), ("slow_turns", C.c_double)]
+
+
+class KvCacheC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p),
+                ("dtype", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("pages", C.c_int64), ("page_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64), ("v_token_stride", C.c_int64),
+                ("v_head_stride", C.c_int64), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("q_out_token_stride", C.c_int64), ("q_out_head_stride", C.c_int64),
+                ("slots", C.c_void_p), ("positions", C.c_void_p), ("table", C.c_void_p),
+                ("table_rows", C.c_int64), ("tokens", C.c_int64), ("x_dtype", C.c_int32), ("heads", C.c_int32),
+                ("rot_dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p),
+                ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("out_token_stride", C.c_int64),
+                ("out_head_stride", C.c_int64), ("block_table", C.c_void_p), ("block_table_stride", C.c_int64),
+                ("kv_len", C.c_void_p), ("cu_q", C.c_void_p), ("tokens", C.c_int64), ("batch", C.c_int32),
+                ("heads", C.c_int32), ("max_q_len", C.c_int32), ("max_kv_len", C.c_int32), ("max_pages", C.c_int32),
+                ("causal", C.c_int32), ("scale", C.c_float)]
+
+
 # Every symbol include/rg_npu.h declares, with its ctypes signature.
 _vp, _i32, _i64, _u64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
 _f32p, _i64p, _i32p, _i8p = C.POINTER(C.c_float), C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.POINTER(C.c_int8)
@@ -111,6 +144,17 @@ SIGNATURES = {
     "rg_attention_f32": ([_vp, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _vp], _i32),
     "rg_activation_f32": ([_vp, _i64, _i32, _f32, _vp, _vp], _i32),
     "rg_selftest_fast_paths": ([_vp], _i32),
+    "rg_quantize_token_i8": ([_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp], _i32),
+    "rg_gemm_i8_token": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _f32, _vp, _i32, _i64, _vp, _vp], _i32),
+    "rg_linear_i8_token_workspace_size": ([_i64, _i64], _i64),
+    "rg_linear_i8_token": ([_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _f32, _vp, _i32, _i64, _vp,
+                            _vp, _vp], _i32),
+    "rg_rope_table_f32": ([C.POINTER(RopeScaling), _i64, _i32, _vp, _vp], _i32),
+    "rg_rope": ([_vp, _i32, _i64, _i32, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp, _vp],
+                _i32),
+    "rg_kv_append": ([C.POINTER(KvCacheC), C.POINTER(KvAppendArgs), _vp, _vp], _i32),
+    "rg_attention_paged_workspace_size": ([C.POINTER(KvCacheC), C.POINTER(PagedAttentionArgs)], _i64),
+    "rg_attention_paged": ([C.POINTER(KvCacheC), C.POINTER(PagedAttentionArgs), _vp, _vp, _vp], _i32),
     "rg_rng_seed": ([C.POINTER(RngC), _u64], None),
     "rg_rng_next_u64": ([C.POINTER(RngC)], _u64),
     "rg_rng_fill_uniform": ([C.POINTER(RngC), _f32p, _i64, _f32, _f32], None),

@@ -2556,7 +2556,8 @@ rg_status rg_gemm_i8_fused(const int8_t* a, const int8_t* w, int64_t m, int64_t 
 rg_status rg_status_from_error_words(const int32_t words[2]) {
   if (!words) return fail(RG_ERR_INVALID_ARG, "null argument");
   if (words[0]) return fail(RG_ERR_TIMEOUT, "a tensor-core kernel gave up on a bounded wait; results are invalid");
-  if (words[1]) return fail(RG_ERR_INVALID_ARG, "Embedding: a token id is not below the vocabulary size");
+  if (words[1]) return fail(RG_ERR_INVALID_ARG, "an index is out of range: an Embedding token id not below the "
+                                    "vocabulary size, or a serving call's position, slot, page or length");
   return RG_OK;
 }
 

@@ -1,0 +1,109 @@
+// rg_serving.h -- launchers of the decoder-serving kernels (internal to librg_npu.so) and
+// the element types they share.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/rg_npu.h"
+
+namespace rg {
+
+inline int dtype_size(int32_t dt) { return dt == RG_DTYPE_F32 ? 4 : 2; }
+
+template <typename T>
+struct ElemOf;  // conversions to and from f32, one rounding each (none widening)
+template <>
+struct ElemOf<float> {
+  static __device__ __forceinline__ float to(float v) { return v; }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <>
+struct ElemOf<__half> {
+  static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
+template <>
+struct ElemOf<__nv_bfloat16> {
+  static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
+
+// N consecutive elements as f32, moved 16 bytes at a time (or all at once when shorter):
+// the address is aligned to min(16, N * sizeof(T)).
+template <typename T, int N>
+struct Pack {
+  static constexpr int kBytes = N * (int)sizeof(T);
+  static constexpr int kWord = kBytes >= 16 ? 16 : kBytes;
+  struct alignas(kWord) Word {
+    T e[kWord / (int)sizeof(T)];
+  };
+  static constexpr int kPer = kWord / (int)sizeof(T);
+  static __device__ __forceinline__ void load(const T* p, float (&f)[N]) {
+#pragma unroll
+    for (int w = 0; w < N / kPer; ++w) {
+      const Word v = reinterpret_cast<const Word*>(p)[w];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) f[w * kPer + i] = ElemOf<T>::to(v.e[i]);
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[N]) {
+#pragma unroll
+    for (int w = 0; w < N / kPer; ++w) {
+      Word v;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v.e[i] = ElemOf<T>::from(f[w * kPer + i]);
+      reinterpret_cast<Word*>(p)[w] = v;
+    }
+  }
+};
+
+// ---- per-token linear (k_linear_token.cu) ---------------------------------------
+void launch_quantize_token(const void* x, int32_t dtype, int64_t rows, int64_t k, int64_t ldx, int8_t* q, int64_t ldq,
+                           float* scale, cudaStream_t st);
+struct TokenGemmArgs {
+  const int8_t* a = nullptr;       // [m, ld]
+  const float* a_scale = nullptr;  // [m]
+  const int8_t* w = nullptr;       // [n, ld]
+  const float* w_scale = nullptr;  // [n]
+  const float* bias = nullptr;     // [n] or NULL
+  int64_t m = 0, n = 0, ld = 0, ldo = 0;
+  int32_t act = 0;
+  float act_param = 0.0f;
+  void* out = nullptr;
+  int32_t out_dtype = 0;
+  int32_t* err = nullptr;
+};
+rg_status launch_gemm_token(const TokenGemmArgs& a, cudaStream_t st);
+
+// ---- rotary positions and the paged append (k_rope.cu) --------------------------
+// Three groups of heads per token: q heads (rotated, stored by strides), then kv_heads
+// key heads (rotated, stored in the cache) and kv_heads value heads (copied there).
+struct RopeArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  int64_t q_ts = 0, q_hs = 0, k_ts = 0, k_hs = 0, v_ts = 0, v_hs = 0;
+  void *q_out = nullptr, *k_out = nullptr, *v_out = nullptr;
+  int64_t qo_ts = 0, qo_hs = 0, page_stride = 0, token_stride = 0, head_stride = 0;
+  const int32_t* positions = nullptr;
+  const float* table = nullptr;
+  const int64_t* slots = nullptr;
+  int64_t table_rows = 0, tokens = 0, num_slots = 0;
+  int32_t heads = 0, kv_heads = 0, head_dim = 0, rot_dim = 0, page_size = 1;
+  int32_t in_dtype = 0, out_dtype = 0, interleaved = 0;
+  int32_t* err = nullptr;
+};
+rg_status launch_rope(const RopeArgs& a, cudaStream_t st);
+void launch_rope_table(const rg_rope_scaling& s, int64_t positions, int32_t rot_dim, float* table, cudaStream_t st);
+
+// ---- attention over a paged cache (k_attn_paged.cu) ------------------------------
+struct PagedAttnArgs {
+  rg_kv_cache c;
+  rg_paged_attention_args a;
+  void* workspace = nullptr;
+  int32_t* err = nullptr;
+};
+int64_t attention_paged_workspace(const PagedAttnArgs& a);
+rg_status launch_attention_paged(const PagedAttnArgs& a, cudaStream_t st);
+
+}  // namespace rg
