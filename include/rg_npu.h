@@ -365,13 +365,16 @@ rg_status rg_gemm_i8_token(const int8_t* a, const float* a_scale, const int8_t* 
                            int64_t n, int64_t ld, const float* bias, int32_t act, float act_param, void* out,
                            int32_t out_dtype, int64_t ldo, int32_t* error_words, void* stream);
 /* The two in one call: x [m, k] (row stride ldx) against w [n, ld], ld >= k.  `workspace`
- * holds rg_linear_i8_token_workspace_size(m, ld) bytes, 256-byte aligned, and is free
- * again once the call's work on `stream` is done. */
+ * holds rg_linear_i8_token_workspace_size(m, ld) bytes, 256-byte aligned (NULL when that is
+ * 0), and is free again once the call's work on `stream` is done. */
+typedef struct rg_linear_token_args {
+  const void* x; const int8_t* w; const float* w_scale; const float* bias; void* out;
+  int64_t m, k, ldx, n, ld, ldo;
+  int32_t x_dtype, out_dtype, act;
+  float act_param;
+} rg_linear_token_args;
 int64_t rg_linear_i8_token_workspace_size(int64_t m, int64_t ld);
-rg_status rg_linear_i8_token(const void* x, int32_t x_dtype, int64_t m, int64_t k, int64_t ldx, const int8_t* w,
-                             const float* w_scale, int64_t n, int64_t ld, const float* bias, int32_t act,
-                             float act_param, void* out, int32_t out_dtype, int64_t ldo, void* workspace,
-                             int32_t* error_words, void* stream);
+rg_status rg_linear_i8_token(const rg_linear_token_args* args, void* workspace, int32_t* error_words, void* stream);
 
 /* Rotary positions.  A table has one f32 row per position: rot_dim / 2 cosines, then
  * rot_dim / 2 sines, of position * freq[i].  With freq[i] = base^(-2 i / rot_dim):
@@ -395,10 +398,15 @@ rg_status rg_rope_table_f32(const rg_rope_scaling* scaling, int64_t positions, i
  * (a, b) -> (a c - b s, b c + a s), with a, b dimensions i and i + rot_dim / 2, or 2 i and
  * 2 i + 1 when `interleaved`.  x, out: [tokens, heads, head_dim], head_dim contiguous, the
  * other strides in elements; out may be x (with the same strides).  Sums in f32. */
-rg_status rg_rope(const void* x, int32_t dtype, int64_t tokens, int32_t heads, int32_t head_dim,
-                  int64_t token_stride, int64_t head_stride, const int32_t* positions, const float* table,
-                  int64_t table_rows, int32_t rot_dim, int32_t interleaved, void* out, int64_t out_token_stride,
-                  int64_t out_head_stride, int32_t* error_words, void* stream);
+typedef struct rg_rope_args {
+  const void* x; void* out;
+  int64_t token_stride, head_stride, out_token_stride, out_head_stride;
+  const int32_t* positions;
+  const float* table;
+  int64_t table_rows, tokens;
+  int32_t dtype, heads, head_dim, rot_dim, interleaved;
+} rg_rope_args;
+rg_status rg_rope(const rg_rope_args* args, int32_t* error_words, void* stream);
 
 /* One layer's paged cache: `pages` pages of page_size tokens, keys and values in two
  * tensors with the same strides (elements), head_dim contiguous; dtype f16 or bf16. */

@@ -181,6 +181,48 @@ pub struct rg_rope_scaling {
     pub slow_turns: double,
 }
 
+/// One call of `rg_linear_i8_token`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rg_linear_token_args {
+    pub x: *const c_void,
+    pub w: *const i8,
+    pub w_scale: *const f32,
+    pub bias: *const f32,
+    pub out: *mut c_void,
+    pub m: i64,
+    pub k: i64,
+    pub ldx: i64,
+    pub n: i64,
+    pub ld: i64,
+    pub ldo: i64,
+    pub x_dtype: i32,
+    pub out_dtype: i32,
+    pub act: i32,
+    pub act_param: f32,
+}
+
+/// One call of `rg_rope`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rg_rope_args {
+    pub x: *const c_void,
+    pub out: *mut c_void,
+    pub token_stride: i64,
+    pub head_stride: i64,
+    pub out_token_stride: i64,
+    pub out_head_stride: i64,
+    pub positions: *const i32,
+    pub table: *const f32,
+    pub table_rows: i64,
+    pub tokens: i64,
+    pub dtype: i32,
+    pub heads: i32,
+    pub head_dim: i32,
+    pub rot_dim: i32,
+    pub interleaved: i32,
+}
+
 /// One layer's paged key / value cache.
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -317,16 +359,11 @@ extern "C" {
                             n: i64, ld: i64, bias: *const f32, act: i32, act_param: f32, out: *mut c_void,
                             out_dtype: i32, ldo: i64, error_words: *mut i32, stream: *mut c_void) -> rg_status;
     pub fn rg_linear_i8_token_workspace_size(m: i64, ld: i64) -> i64;
-    pub fn rg_linear_i8_token(x: *const c_void, x_dtype: i32, m: i64, k: i64, ldx: i64, w: *const i8,
-                              w_scale: *const f32, n: i64, ld: i64, bias: *const f32, act: i32,
-                              act_param: f32, out: *mut c_void, out_dtype: i32, ldo: i64,
-                              workspace: *mut c_void, error_words: *mut i32, stream: *mut c_void) -> rg_status;
+    pub fn rg_linear_i8_token(args: *const rg_linear_token_args, workspace: *mut c_void, error_words: *mut i32,
+                              stream: *mut c_void) -> rg_status;
     pub fn rg_rope_table_f32(scaling: *const rg_rope_scaling, positions: i64, rot_dim: i32, table: *mut f32,
                              stream: *mut c_void) -> rg_status;
-    pub fn rg_rope(x: *const c_void, dtype: i32, tokens: i64, heads: i32, head_dim: i32, token_stride: i64,
-                   head_stride: i64, positions: *const i32, table: *const f32, table_rows: i64, rot_dim: i32,
-                   interleaved: i32, out: *mut c_void, out_token_stride: i64, out_head_stride: i64,
-                   error_words: *mut i32, stream: *mut c_void) -> rg_status;
+    pub fn rg_rope(args: *const rg_rope_args, error_words: *mut i32, stream: *mut c_void) -> rg_status;
     pub fn rg_kv_append(cache: *const rg_kv_cache, args: *const rg_kv_append_args, error_words: *mut i32,
                         stream: *mut c_void) -> rg_status;
     pub fn rg_attention_paged_workspace_size(cache: *const rg_kv_cache,

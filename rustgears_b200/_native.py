@@ -78,6 +78,20 @@ class RopeScaling(C.Structure):
                 ("old_context", C.c_double), ("fast_turns", C.c_double), ("slow_turns", C.c_double)]
 
 
+class LinearTokenArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("w_scale", C.c_void_p), ("bias", C.c_void_p),
+                ("out", C.c_void_p), ("m", C.c_int64), ("k", C.c_int64), ("ldx", C.c_int64), ("n", C.c_int64),
+                ("ld", C.c_int64), ("ldo", C.c_int64), ("x_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("act", C.c_int32), ("act_param", C.c_float)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("positions", C.c_void_p),
+                ("table", C.c_void_p), ("table_rows", C.c_int64), ("tokens", C.c_int64), ("dtype", C.c_int32),
+                ("heads", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
 class KvCacheC(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p),
                 ("dtype", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
@@ -147,14 +161,13 @@ SIGNATURES = {
     "rg_quantize_token_i8": ([_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp], _i32),
     "rg_gemm_i8_token": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _f32, _vp, _i32, _i64, _vp, _vp], _i32),
     "rg_linear_i8_token_workspace_size": ([_i64, _i64], _i64),
-    "rg_linear_i8_token": ([_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _f32, _vp, _i32, _i64, _vp,
-                            _vp, _vp], _i32),
+    "rg_linear_i8_token": ([_vp, _vp, _vp, _vp], _i32),
     "rg_rope_table_f32": ([C.POINTER(RopeScaling), _i64, _i32, _vp, _vp], _i32),
-    "rg_rope": ([_vp, _i32, _i64, _i32, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp, _vp],
-                _i32),
-    "rg_kv_append": ([C.POINTER(KvCacheC), C.POINTER(KvAppendArgs), _vp, _vp], _i32),
-    "rg_attention_paged_workspace_size": ([C.POINTER(KvCacheC), C.POINTER(PagedAttentionArgs)], _i64),
-    "rg_attention_paged": ([C.POINTER(KvCacheC), C.POINTER(PagedAttentionArgs), _vp, _vp, _vp], _i32),
+    # argument structs come packed (a bytes object) or as ctypes structures by reference
+    "rg_rope": ([_vp, _vp, _vp], _i32),
+    "rg_kv_append": ([_vp, _vp, _vp, _vp], _i32),
+    "rg_attention_paged_workspace_size": ([_vp, _vp], _i64),
+    "rg_attention_paged": ([_vp, _vp, _vp, _vp, _vp], _i32),
     "rg_rng_seed": ([C.POINTER(RngC), _u64], None),
     "rg_rng_next_u64": ([C.POINTER(RngC)], _u64),
     "rg_rng_fill_uniform": ([C.POINTER(RngC), _f32p, _i64, _f32, _f32], None),

@@ -1,76 +1,407 @@
-// k_attn_paged.cu -- attention of a chunk of new tokens over a paged cache.
+// k_attn_paged.cu -- attention of a chunk of new tokens over a paged cache: the kernel for
+// few rows (decoding), and for the shapes the tcgen05 kernel does not take.
 //
 // Query i of sequence b (of q_len, with kv_len keys) sees keys j <= kv_len - q_len + i:
-//   o = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s),  s_j = scale * q . k_j,
+//   o = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  s_j = scale log2(e) q . k_j,  m = max s_j,
 // one pass over the keys with the running maximum and sum; a row without keys is zeros.
+//
+// Rows: the heads / kv_heads query heads that share a key head are rows of one matrix
+// product, row r = token r / group, head r % group, so a key is read once for all of them.
+// A block takes 16 WR rows of one (sequence, key head) and a share of its keys; its warps
+// are WR row groups x WK key groups, each 16 rows x its keys of every tile, with its
+// own maximum, sum and output (registers), joined once at the end.
+//
+// Bound: memory for few rows (keys and values are read once: 4 head_dim bytes per key and
+// key head; 16 rows fill one m16n8k16 fragment, whose rate is far above what the loads
+// need).  A three-stage ring of cp.async tiles keeps two tiles in flight per block.
+// Few (sequence, head) pairs leave SMs idle, so a sequence's keys are split over a cluster
+// of up to 16 blocks that join their partial rows through distributed shared memory: no
+// second launch and no workspace, and the same order of additions in every run.
+#include <cooperative_groups.h>
+
+#include <climits>
+
+#include "rg_mma16.cuh"
 #include "rg_serving.h"
 
 namespace rg {
 namespace {
 
-// One warp per query row (token, head); lane l holds dimensions l, l + 32, ...
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_attn_rows(const PagedAttnArgs p) {
-  const rg_kv_cache& c = p.c;
-  const rg_paged_attention_args& a = p.a;
-  const int lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
+namespace cg = cooperative_groups;
+using namespace mma16;
+
+constexpr int kStages = 3;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// n / d for 0 <= n < 2^31 by multiplication (Granlund and Montgomery, PLDI 1994):
+// m = floor(2^32 (2^l - d) / d) + 1, l = ceil(log2 d).
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t v = 1) : d(v) {
+    uint32_t l = 0;
+    while ((1ull << l) < v) ++l;
+    m = (uint32_t)(((1ull << 32) * ((1ull << l) - v)) / v + 1);
+    s = l;
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return (uint32_t)(((uint64_t)__umulhi(n, m) + n) >> s);
+  }
+};
+
+struct Params {
+  PagedAttnArgs p;
+  FastDiv page, group;
+  int32_t splits, tiles;  // blocks over a sequence's keys, and over its rows
+  float scale2;           // scale * log2(e)
+};
+
+template <int D, int WR, int WK>
+struct Shape {
+  static constexpr int KT = D <= 128 ? 64 : 32;    // keys of a tile: two blocks' rings fit an SM
+  static constexpr int kWarps = WR * WK, kThreads = 32 * kWarps, kRows = 16 * WR;
+  static constexpr int kKeys = KT / WK;            // keys of a warp in a tile
+  static constexpr int kPitch = D * 2 + 16;        // odd multiple of 16 bytes: ldmatrix without conflicts
+  static constexpr int kTile = KT * kPitch;
+  static constexpr int kStage = 2 * kTile;         // keys, values
+  static constexpr int kQ = kRows * kPitch;
+  static constexpr int kOffs = (kStages + 1) * KT * 8;
+  static constexpr int kSmem = kQ + kStages * kStage + kOffs;
+  static constexpr bool kQRegs = D <= 128;         // query fragments stay in registers
+  // the join reuses the ring: kRows x (D + 4) outputs, then per-warp maxima and sums
+  static constexpr int kOPitch = D + 4;
+  static_assert(kRows * kOPitch * 4 + 2 * (kWarps + 1) * 16 * WR * 4 <= kStages * kStage, "join fits the ring");
+};
+
+template <typename T, int D, int WR, int WK>
+__global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
+  using S = Shape<D, WR, WK>;
+  constexpr int KT = S::KT;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const rg_kv_cache& c = P.p.c;
+  const rg_paged_attention_args& a = P.p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wr = warp % WR, wk = warp / WR;
+  const int split = blockIdx.x % P.splits, tile = blockIdx.x / P.splits;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int group = P.group.d;
+
+  uint8_t* sq = smem;
+  uint8_t* ring = smem + S::kQ;
+  int64_t* offs = reinterpret_cast<int64_t*>(ring + kStages * S::kStage);  // [kStages + 1][KT], -1: zeros
+
+  // The same for every block of a cluster, so that all of them leave or stay together.
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int kv = a.kv_len[b];
   if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) {
-    if (threadIdx.x == 0) p.err[1] = 1;
+    if (tid == 0) P.p.err[1] = 1;
     return;
   }
-  const int ql = (int)(q1 - q0);
-  if (i >= ql) return;
-  const int hk = h / (a.heads / c.kv_heads);
-  constexpr int N = D / 32;
-  float q[N], o[N];
-  const T* qp = static_cast<const T*>(a.q) + (q0 + i) * a.q_token_stride + h * a.q_head_stride;
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    q[j] = ElemOf<T>::to(qp[lane + 32 * j]) * a.scale;
-    o[j] = 0.0f;
+  const int ql = (int)(q1 - q0), rows = ql * group, row0 = tile * S::kRows;
+  if (row0 >= rows) return;
+  // keys seen by the tile's last row
+  const int last_tok = (int)P.group.div((uint32_t)(min(row0 + S::kRows, rows) - 1));
+  const int seen = a.causal ? max(0, min(kv, kv - ql + last_tok + 1)) : kv;
+  const int n_tiles = (seen + KT - 1) / KT;
+  const int per = (n_tiles + P.splits - 1) / P.splits;
+  const int t0 = min(split * per, n_tiles), t1 = min(t0 + per, n_tiles);
+
+  // ---- queries: rows past the last one are zeros ----
+  for (int i = tid; i < S::kRows * (D / 8); i += S::kThreads) {
+    const int r = i / (D / 8), ch = i % (D / 8), row = row0 + r;
+    const bool ok = row < rows;
+    const int tok = (int)P.group.div((uint32_t)(ok ? row : 0)), h = hk * group + (ok ? row : 0) - tok * group;
+    cp_async16(saddr(sq + r * S::kPitch + ch * 16),
+               static_cast<const T*>(a.q) + (q0 + tok) * a.q_token_stride + h * a.q_head_stride + ch * 8, ok);
   }
-  float top = -INFINITY, sum = 0.0f;
-  const int last = a.causal ? min(kv, kv - ql + i + 1) : kv;  // keys seen
-  for (int key = 0; key < last; ++key) {
-    const int page = a.block_table[(int64_t)b * a.block_table_stride + key / c.page_size];
-    const bool ok = page >= 0 && page < c.pages;
-    if (!ok && lane == 0) p.err[1] = 1;
-    const int64_t at = ok ? page * c.page_stride + (key % c.page_size) * c.token_stride + hk * c.head_stride : 0;
-    float s = 0.0f;
+  cp_async_commit();
+
+  // ---- key addresses: thread r < KT looks tile t's key r up, one tile ahead of its loads ----
+  const auto look = [&](int t) -> int64_t {
+    const int key = t * KT + tid;
+    if (t >= t1 || key >= seen) return -1;
+    const uint32_t pi = P.page.div((uint32_t)key);
+    const int64_t page = a.block_table[(int64_t)b * a.block_table_stride + pi];
+    if (page < 0 || page >= c.pages) {
+      P.p.err[1] = 1;
+      return -1;
+    }
+    return page * c.page_stride + (int64_t)(key - pi * c.page_size) * c.token_stride + hk * c.head_stride;
+  };
+  const auto load = [&](int t) {  // tile t into its stage
+    const int stage = (t - t0) % kStages;
+    const int64_t* off = offs + ((t - t0) % (kStages + 1)) * KT;
+    const uint32_t base = saddr(ring + stage * S::kStage);
+#pragma unroll 4
+    for (int i = tid; i < KT * (D / 8); i += S::kThreads) {
+      const int r = i / (D / 8), ch = i % (D / 8);
+      const int64_t o = off[r];
+      const bool ok = o >= 0;
+      const int64_t at = ok ? o + ch * 8 : 0;
+      cp_async16(base + r * S::kPitch + ch * 16, static_cast<const T*>(c.k) + at, ok);
+      cp_async16(base + S::kTile + r * S::kPitch + ch * 16, static_cast<const T*>(c.v) + at, ok);
+    }
+  };
+  if (tid < KT)
+    for (int s = 0; s < kStages; ++s) offs[s * KT + tid] = look(t0 + s);
+  __syncthreads();
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (t0 + s < t1) load(t0 + s);
+    cp_async_commit();
+  }
+  int64_t ahead = tid < KT ? look(t0 + kStages) : -1;
+
+  // ---- main loop ----
+  const int g = lane >> 2, t4 = lane & 3;
+  int limit[2];  // keys seen by this thread's two rows (g, g + 8)
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      s = fmaf(q[j], ok ? ElemOf<T>::to(static_cast<const T*>(c.k)[at + lane + 32 * j]) : 0.0f, s);
+  for (int i = 0; i < 2; ++i) {
+    const int row = row0 + wr * 16 + g + 8 * i;
+    limit[i] = row >= rows ? 0 : a.causal ? min(kv, kv - ql + (int)P.group.div((uint32_t)row) + 1) : kv;
+  }
+  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float m = fmaxf(top, s);
-    const float keep = m == -INFINITY ? 1.0f : expf(top - m);
-    const float e = m == -INFINITY ? 0.0f : expf(s - m);
-    sum = fmaf(sum, keep, e);
-    top = m;
+  for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float v = ok ? ElemOf<T>::to(static_cast<const T*>(c.v)[at + lane + 32 * j]) : 0.0f;
-      o[j] = fmaf(o[j], keep, e * v);
+    for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
+  uint32_t qf[S::kQRegs ? D / 16 : 1][4];
+  const uint32_t q_addr = saddr(sq + (wr * 16 + (lane & 15)) * S::kPitch + (lane >> 4) * 16);
+
+  for (int t = t0; t < t1; ++t) {
+    cp_async_wait<kStages - 2>();
+    if (tid < KT) {
+      offs[((t - t0 + kStages) % (kStages + 1)) * KT + tid] = ahead;
+      ahead = look(t + kStages + 1);
+    }
+    __syncthreads();  // tile t has landed, and everyone is done with tile t - 1's stage
+    if (t + kStages - 1 < t1) load(t + kStages - 1);
+    cp_async_commit();
+    if constexpr (S::kQRegs) {
+      if (t == t0)
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) ldmatrix4(qf[d], q_addr + d * 32);
+    }
+    const uint32_t kb = saddr(ring + ((t - t0) % kStages) * S::kStage) + wk * S::kKeys * S::kPitch;
+    const uint32_t vb = kb + S::kTile;
+    // scores: fragments of 8 keys
+    float s[S::kKeys / 8][4];
+#pragma unroll
+    for (int j = 0; j < S::kKeys / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[j][i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      if constexpr (!S::kQRegs) ldmatrix4(qf[0], q_addr + d * 32);
+#pragma unroll
+      for (int j = 0; j < S::kKeys / 16; ++j) {
+        uint32_t kf[4];  // keys 16 j .. + 7 (dims 0-7, 8-15), then the next 8 keys
+        ldmatrix4(kf, kb + (j * 16 + (lane & 7) + ((lane >> 4) << 3)) * S::kPitch + d * 32 + ((lane >> 3) & 1) * 16);
+        mma<T>(s[2 * j], qf[S::kQRegs ? d : 0], kf[0], kf[1]);
+        mma<T>(s[2 * j + 1], qf[S::kQRegs ? d : 0], kf[2], kf[3]);
+      }
+    }
+    const int key0 = t * KT + wk * S::kKeys + 2 * t4;
+    float top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int j = 0; j < S::kKeys / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = s[j][i] * P.scale2;
+        s[j][i] = key0 + j * 8 + (i & 1) < limit[i >> 1] ? v : -INFINITY;
+        top[i >> 1] = fmaxf(top[i >> 1], s[j][i]);
+      }
+    float base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      base[i] = top[i] == -INFINITY ? 0.0f : top[i];  // no key yet: 2^(-inf - 0) = 0
+    }
+    if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+      const float f0 = ex2(m[0] - base[0]), f1 = ex2(m[1] - base[1]);
+      l[0] *= f0;
+      l[1] *= f1;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        o[j][0] *= f0;
+        o[j][1] *= f0;
+        o[j][2] *= f1;
+        o[j][3] *= f1;
+      }
+      m[0] = top[0];
+      m[1] = top[1];
+    }
+#pragma unroll
+    for (int j = 0; j < S::kKeys / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[j][i] = ex2(s[j][i] - base[i >> 1]);
+        l[i >> 1] += s[j][i];
+      }
+    // output: the probabilities, rounded to the cache's type, times the values
+#pragma unroll
+    for (int j = 0; j < S::kKeys / 16; ++j) {
+      const uint32_t pf[4] = {pack<T>(s[2 * j][0], s[2 * j][1]), pack<T>(s[2 * j][2], s[2 * j][3]),
+                              pack<T>(s[2 * j + 1][0], s[2 * j + 1][1]), pack<T>(s[2 * j + 1][2], s[2 * j + 1][3])};
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t vf[4];  // dims 16 d .. + 7 (keys 0-7, 8-15), then the next 8 dims
+        ldmatrix4_trans(vf, vb + (j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * S::kPitch + d * 32 + (lane >> 4) * 16);
+        mma<T>(o[2 * d], pf, vf[0], vf[1]);
+        mma<T>(o[2 * d + 1], pf, vf[2], vf[3]);
+      }
     }
   }
-  T* op = static_cast<T*>(a.out) + (q0 + i) * a.out_token_stride + h * a.out_head_stride;
 #pragma unroll
-  for (int j = 0; j < N; ++j) op[lane + 32 * j] = ElemOf<T>::from(sum > 0.0f ? o[j] / sum : 0.0f);
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+  }
+
+  // ---- join the key groups: every warp scales to the rows' common maximum, adds in order ----
+  cp_async_wait<0>();
+  __syncthreads();
+  float* jo = reinterpret_cast<float*>(ring);          // [kRows][kOPitch]
+  float* jm = jo + S::kRows * S::kOPitch;              // [WK][kRows], then the joined [kRows]
+  float* jl = jm + (S::kWarps + 1) * 16 * WR;
+  const int r0 = wr * 16 + g;
+  if (t4 == 0)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      jm[wk * S::kRows + r0 + 8 * i] = m[i];
+      jl[wk * S::kRows + r0 + 8 * i] = l[i];
+    }
+  __syncthreads();
+  float f[2], M[2], L[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    M[i] = -INFINITY;
+    L[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) M[i] = fmaxf(M[i], jm[w * S::kRows + r0 + 8 * i]);
+    const float base = M[i] == -INFINITY ? 0.0f : M[i];
+#pragma unroll
+    for (int w = 0; w < WK; ++w) L[i] += jl[w * S::kRows + r0 + 8 * i] * ex2(jm[w * S::kRows + r0 + 8 * i] - base);
+    f[i] = ex2(m[i] - base);
+  }
+  for (int w = 0; w < WK; ++w) {
+    if (wk == w)
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float2* dst = reinterpret_cast<float2*>(jo + (r0 + 8 * i) * S::kOPitch + j * 8 + 2 * t4);
+          float2 v = w == 0 ? make_float2(0.0f, 0.0f) : *dst;
+          v.x += o[j][2 * i] * f[i];
+          v.y += o[j][2 * i + 1] * f[i];
+          *dst = v;
+        }
+    __syncthreads();
+  }
+  float* fm = jm + WK * S::kRows;  // the block's maxima and sums
+  float* fl = jl + WK * S::kRows;
+  if (wk == 0 && t4 == 0)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      fm[r0 + 8 * i] = M[i];
+      fl[r0 + 8 * i] = L[i];
+    }
+
+  // ---- join the splits, normalise, store: block `split` of the cluster takes a share ----
+  const auto store = [&](int r, int ch, float (&v)[8], float sum) {
+    const int row = row0 + r;
+    if (row >= rows) return;
+    const int tok = (int)P.group.div((uint32_t)row), h = hk * group + row - tok * group;
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = sum == 0.0f ? 0.0f : v[i] * inv;  // no key: zeros
+    Pack<T, 8>::store(static_cast<T*>(a.out) + (q0 + tok) * a.out_token_stride + h * a.out_head_stride + ch * 8, v);
+  };
+  if (P.splits == 1) {
+    __syncthreads();
+    for (int i = tid; i < S::kRows * (D / 8); i += S::kThreads) {
+      const int r = i / (D / 8), ch = i % (D / 8);
+      float v[8];
+      Pack<float, 8>::load(jo + r * S::kOPitch + ch * 8, v);
+      store(r, ch, v, fl[r]);
+    }
+    return;
+  }
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  for (int i = split * S::kThreads + tid; i < S::kRows * (D / 8); i += P.splits * S::kThreads) {
+    const int r = i / (D / 8), ch = i % (D / 8);
+    float top = -INFINITY, sum = 0.0f, v[8];
+    for (int w = 0; w < P.splits; ++w) top = fmaxf(top, cl.map_shared_rank(fm, w)[r]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    for (int w = 0; w < P.splits; ++w) {
+      const float e = ex2(cl.map_shared_rank(fm, w)[r] - base);
+      sum += e * cl.map_shared_rank(fl, w)[r];
+      float x[8];
+      Pack<float, 8>::load(cl.map_shared_rank(jo, w) + r * S::kOPitch + ch * 8, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += e * x[j];
+    }
+    store(r, ch, v, sum);
+  }
+  cl.sync();  // no block leaves while another reads its shared memory
+}
+
+template <typename T, int D, int WR, int WK>
+rg_status go(const PagedAttnArgs& p, cudaStream_t st) {
+  using S = Shape<D, WR, WK>;
+  const auto kernel = k_attn_few<T, D, WR, WK>;
+  static DeviceOnce once;
+  once.run([&] {  // a failure shows in the launch
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
+  Params P;
+  P.p = p;
+  P.page = FastDiv((uint32_t)p.c.page_size);
+  P.group = FastDiv((uint32_t)(p.a.heads / p.c.kv_heads));
+  P.scale2 = p.a.scale * kLog2e;
+  const int64_t rows = (int64_t)p.a.max_q_len * P.group.d;
+  const int64_t tiles = (rows + S::kRows - 1) / S::kRows;
+  if (rows > INT_MAX || p.c.kv_heads > 65535) return RG_ERR_UNSUPPORTED;
+  // Splits: enough blocks to fill two per SM four times over (unequal lengths even out), while
+  // every split keeps two tiles.
+  const int64_t blocks = tiles * p.c.kv_heads * p.a.batch;
+  int splits = 1;
+  while (splits < 16 && blocks * splits < 148 * 8 && (int64_t)splits * 2 * 2 * S::KT <= p.a.max_kv_len) splits *= 2;
+  if (tiles * splits > INT_MAX) return RG_ERR_UNSUPPORTED;
+  P.splits = splits;
+  P.tiles = (int32_t)tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * splits), (unsigned)p.c.kv_heads, (unsigned)p.a.batch);
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, P);
+  return RG_OK;
+}
+
+template <typename T, int D>
+rg_status go_rows(const PagedAttnArgs& p, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.a.max_q_len * (p.a.heads / p.c.kv_heads);
+  return rows <= 16 ? go<T, D, 1, (D <= 128 ? 4 : 2)>(p, st) : go<T, D, 4, 2>(p, st);
 }
 
 template <typename T>
-rg_status go(const PagedAttnArgs& p, cudaStream_t st) {
-  const dim3 grid((unsigned)((p.a.max_q_len + 3) / 4), (unsigned)p.a.heads, (unsigned)p.a.batch);
+rg_status go_dim(const PagedAttnArgs& p, cudaStream_t st) {
   switch (p.c.head_dim) {
-    case 64: k_attn_rows<T, 64><<<grid, 128, 0, st>>>(p); break;
-    case 96: k_attn_rows<T, 96><<<grid, 128, 0, st>>>(p); break;
-    case 128: k_attn_rows<T, 128><<<grid, 128, 0, st>>>(p); break;
-    default: k_attn_rows<T, 256><<<grid, 128, 0, st>>>(p); break;
+    case 64: return go_rows<T, 64>(p, st);
+    case 96: return go_rows<T, 96>(p, st);
+    case 128: return go_rows<T, 128>(p, st);
+    default: return go_rows<T, 256>(p, st);
   }
-  return RG_OK;
 }
 
 }  // namespace
@@ -78,7 +409,7 @@ rg_status go(const PagedAttnArgs& p, cudaStream_t st) {
 int64_t attention_paged_workspace(const PagedAttnArgs&) { return 0; }
 
 rg_status launch_attention_paged(const PagedAttnArgs& p, cudaStream_t st) {
-  return p.c.dtype == RG_DTYPE_F16 ? go<__half>(p, st) : go<__nv_bfloat16>(p, st);
+  return p.c.dtype == RG_DTYPE_F16 ? go_dim<__half>(p, st) : go_dim<__nv_bfloat16>(p, st);
 }
 
 }  // namespace rg

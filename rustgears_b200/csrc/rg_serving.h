@@ -6,9 +6,29 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/rg_npu.h"
 
 namespace rg {
+
+// Runs a kernel's set-up once on every device (a function attribute belongs to the device
+// that was current).
+class DeviceOnce {
+ public:
+  template <typename F>
+  void run(F f) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev > 63) return f();
+    const uint64_t bit = 1ull << dev;
+    if (done_.load(std::memory_order_acquire) & bit) return;
+    f();
+    done_.fetch_or(bit, std::memory_order_release);
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 inline int dtype_size(int32_t dt) { return dt == RG_DTYPE_F32 ? 4 : 2; }
 

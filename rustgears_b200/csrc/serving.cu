@@ -130,23 +130,22 @@ int64_t rg_linear_i8_token_workspace_size(int64_t m, int64_t ld) {
   return round_up(m * ld, 256) + round_up(m * (int64_t)sizeof(float), 256);
 }
 
-rg_status rg_linear_i8_token(const void* x, int32_t x_dtype, int64_t m, int64_t k, int64_t ldx, const int8_t* w,
-                             const float* w_scale, int64_t n, int64_t ld, const float* bias, int32_t act,
-                             float act_param, void* out, int32_t out_dtype, int64_t ldo, void* workspace,
-                             int32_t* error_words, void* stream) {
+rg_status rg_linear_i8_token(const rg_linear_token_args* p, void* workspace, int32_t* error_words, void* stream) {
   const char* f = "rg_linear_i8_token";
-  RG_CHECK(check_gemm(f, w, w_scale, m, n, ld, bias, act, out, out_dtype, ldo, error_words));
-  if (m > 0 && (!workspace || !aligned(workspace, 256)))
+  if (!p) return refuse(RG_ERR_INVALID_ARG, "%s: null arguments", f);
+  RG_CHECK(check_gemm(f, p->w, p->w_scale, p->m, p->n, p->ld, p->bias, p->act, p->out, p->out_dtype, p->ldo,
+                      error_words));
+  if (p->m > 0 && (!workspace || !aligned(workspace, 256)))
     return refuse(RG_ERR_INVALID_ARG, "%s: the workspace must be given and 256-byte aligned", f);
   int8_t* q = static_cast<int8_t*>(workspace);
-  float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(m * ld, 256));
-  RG_CHECK(check_quantize(f, x, x_dtype, m, k, ldx, q, ld, scale));
-  if (m == 0) return RG_OK;
-  launch_quantize_token(x, x_dtype, m, k, ldx, q, ld, scale, (cudaStream_t)stream);
+  float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(p->m * p->ld, 256));
+  RG_CHECK(check_quantize(f, p->x, p->x_dtype, p->m, p->k, p->ldx, q, p->ld, scale));
+  if (p->m == 0) return RG_OK;
+  launch_quantize_token(p->x, p->x_dtype, p->m, p->k, p->ldx, q, p->ld, scale, (cudaStream_t)stream);
   TokenGemmArgs g;
-  g.a = q; g.a_scale = scale; g.w = w; g.w_scale = w_scale; g.bias = bias;
-  g.m = m; g.n = n; g.ld = ld; g.ldo = ldo; g.act = act; g.act_param = act_param;
-  g.out = out; g.out_dtype = out_dtype; g.err = error_words;
+  g.a = q; g.a_scale = scale; g.w = p->w; g.w_scale = p->w_scale; g.bias = p->bias;
+  g.m = p->m; g.n = p->n; g.ld = p->ld; g.ldo = p->ldo; g.act = p->act; g.act_param = p->act_param;
+  g.out = p->out; g.out_dtype = p->out_dtype; g.err = error_words;
   return launched(f, launch_gemm_token(g, (cudaStream_t)stream));
 }
 
@@ -171,27 +170,26 @@ rg_status rg_rope_table_f32(const rg_rope_scaling* s, int64_t positions, int32_t
   return launched(f, RG_OK);
 }
 
-rg_status rg_rope(const void* x, int32_t dtype, int64_t tokens, int32_t heads, int32_t head_dim, int64_t token_stride,
-                  int64_t head_stride, const int32_t* positions, const float* table, int64_t table_rows,
-                  int32_t rot_dim, int32_t interleaved, void* out, int64_t out_token_stride, int64_t out_head_stride,
-                  int32_t* error_words, void* stream) {
+rg_status rg_rope(const rg_rope_args* p, int32_t* error_words, void* stream) {
   const char* f = "rg_rope";
-  if (!is_dtype(dtype)) return refuse(RG_ERR_INVALID_ARG, "%s: unknown dtype %d", f, dtype);
-  if (tokens < 0 || heads <= 0 || head_dim <= 0 || (head_dim & 1))
-    return refuse(RG_ERR_INVALID_ARG, "%s: %lld tokens of %d heads of %d (even)", f, (long long)tokens, heads, head_dim);
-  if (token_stride < 0 || head_stride < 0 || out_token_stride < 0 || out_head_stride < 0)
+  if (!p) return refuse(RG_ERR_INVALID_ARG, "%s: null arguments", f);
+  if (!is_dtype(p->dtype)) return refuse(RG_ERR_INVALID_ARG, "%s: unknown dtype %d", f, p->dtype);
+  if (p->tokens < 0 || p->heads <= 0 || p->head_dim <= 0 || (p->head_dim & 1))
+    return refuse(RG_ERR_INVALID_ARG, "%s: %lld tokens of %d heads of %d (even)", f, (long long)p->tokens, p->heads,
+                  p->head_dim);
+  if (p->token_stride < 0 || p->head_stride < 0 || p->out_token_stride < 0 || p->out_head_stride < 0)
     return refuse(RG_ERR_INVALID_ARG, "%s: negative stride", f);
-  if (tokens == 0) return RG_OK;
-  if (!x || !out || !error_words) return refuse(RG_ERR_INVALID_ARG, "%s: null argument", f);
-  if (!aligned(x, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)))
+  if (p->tokens == 0) return RG_OK;
+  if (!p->x || !p->out || !error_words) return refuse(RG_ERR_INVALID_ARG, "%s: null argument", f);
+  if (!aligned(p->x, dtype_size(p->dtype)) || !aligned(p->out, dtype_size(p->dtype)))
     return refuse(RG_ERR_INVALID_ARG, "%s: misaligned tensor", f);
-  RG_CHECK(check_rotation(f, positions, table, table_rows, rot_dim, head_dim));
+  RG_CHECK(check_rotation(f, p->positions, p->table, p->table_rows, p->rot_dim, p->head_dim));
   RopeArgs r;
-  r.q = x; r.q_ts = token_stride; r.q_hs = head_stride;
-  r.q_out = out; r.qo_ts = out_token_stride; r.qo_hs = out_head_stride;
-  r.positions = positions; r.table = table; r.table_rows = table_rows; r.rot_dim = rot_dim;
-  r.tokens = tokens; r.heads = heads; r.head_dim = head_dim;
-  r.in_dtype = r.out_dtype = dtype; r.interleaved = interleaved; r.err = error_words;
+  r.q = p->x; r.q_ts = p->token_stride; r.q_hs = p->head_stride;
+  r.q_out = p->out; r.qo_ts = p->out_token_stride; r.qo_hs = p->out_head_stride;
+  r.positions = p->positions; r.table = p->table; r.table_rows = p->table_rows; r.rot_dim = p->rot_dim;
+  r.tokens = p->tokens; r.heads = p->heads; r.head_dim = p->head_dim;
+  r.in_dtype = r.out_dtype = p->dtype; r.interleaved = p->interleaved; r.err = error_words;
   return launched(f, launch_rope(r, (cudaStream_t)stream));
 }
 

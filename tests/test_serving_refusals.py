@@ -45,18 +45,29 @@ def test_gemm(change, match, status):
             a["act"], C.c_float(0), a["out"], a["dt"], a["ldo"], a["err"], None)
 
 
-@pytest.mark.parametrize("change,match", [(dict(ws=None), "workspace"), (dict(ws=U), "workspace"), (dict(k=33), "ld"),
-                                          (dict(ldx=3), "ldx"), (dict(xdt=9), "dtype"), (dict(x=None), "null")])
-def test_linear(change, match):
-    a = {**GEMM, **dict(x=A, xdt=0, k=30, ldx=30, ws=A), **change}
-    refused("rg_linear_i8_token", INVALID, match, a["x"], a["xdt"], a["m"], a["k"], a["ldx"], a["w"], a["sw"], a["n"],
-            a["ld"], a["bias"], a["act"], C.c_float(0), a["out"], a["dt"], a["ldo"], a["ws"], a["err"], None)
+def linear(**change):
+    return _native.LinearTokenArgs(**{**dict(x=A, w=A, w_scale=A, bias=A, out=A, m=4, k=30, ldx=30, n=8, ld=32, ldo=8,
+                                             x_dtype=0, out_dtype=0, act=0, act_param=0.0), **change})
+
+
+@pytest.mark.parametrize("change,match,ws", [
+    (dict(k=33), "ld", A), (dict(ldx=3), "ldx", A), (dict(x_dtype=9), "dtype", A), (dict(x=None), "null", A),
+    (dict(w=None), "null", A), (dict(act=9), "activation", A), (dict(ld=40), "16", A), (dict(ldo=7), "ldo", A)])
+def test_linear(change, match, ws):
+    refused("rg_linear_i8_token", INVALID, match, C.byref(linear(**change)), ws, A, None)
+
+
+def test_linear_needs_its_workspace():
+    big = linear(m=300)
+    for ws in (None, U):
+        refused("rg_linear_i8_token", INVALID, "workspace", C.byref(big), ws, A, None)
+    refused("rg_linear_i8_token", INVALID, "null", None, A, A, None)
 
 
 def test_linear_workspace_holds_rows_and_scales():
     L = _native.lib()
     assert L.rg_linear_i8_token_workspace_size(0, 32) == 0
-    assert L.rg_linear_i8_token_workspace_size(3, 32) >= 3 * 32 + 3 * 4
+    assert L.rg_linear_i8_token_workspace_size(300, 32) >= 300 * 32 + 300 * 4
 
 
 @pytest.mark.parametrize("change,match", [
@@ -75,18 +86,23 @@ def test_rope_table_sizes(n, rot, table, match):
             None)
 
 
-ROPE = dict(x=A, dt=2, n=3, h=2, d=64, ts=128, hs=64, pos=A, table=A, rows=10, rot=64, out=A, err=A)
-
-
 @pytest.mark.parametrize("change,match", [
-    (dict(dt=3), "dtype"), (dict(n=-1), "tokens"), (dict(h=0), "heads"), (dict(d=63), "even"), (dict(ts=-1), "stride"),
-    (dict(x=None), "null"), (dict(out=None), "null"), (dict(err=None), "null"), (dict(pos=None), "table"),
-    (dict(table=None), "table"), (dict(rows=0), "table"), (dict(rot=66), "rot_dim"), (dict(rot=3), "even"),
+    (dict(dtype=3), "dtype"), (dict(tokens=-1), "tokens"), (dict(heads=0), "heads"), (dict(head_dim=63), "even"),
+    (dict(token_stride=-1), "stride"), (dict(x=None), "null"), (dict(out=None), "null"), (dict(positions=None), "table"),
+    (dict(table=None), "table"), (dict(table_rows=0), "table"), (dict(rot_dim=66), "rot_dim"), (dict(rot_dim=3), "even"),
     (dict(x=A + 1), "misaligned")])
 def test_rope(change, match):
-    a = {**ROPE, **change}
-    refused("rg_rope", INVALID, match, a["x"], a["dt"], a["n"], a["h"], a["d"], a["ts"], a["hs"], a["pos"], a["table"],
-            a["rows"], a["rot"], 0, a["out"], a["ts"], a["hs"], a["err"], None)
+    a = _native.RopeArgs(**{**dict(x=A, out=A, token_stride=128, head_stride=64, out_token_stride=128,
+                                   out_head_stride=64, positions=A, table=A, table_rows=10, tokens=3, dtype=2, heads=2,
+                                   head_dim=64, rot_dim=64, interleaved=0), **change})
+    refused("rg_rope", INVALID, match, C.byref(a), A, None)
+
+
+def test_rope_needs_error_words():
+    a = _native.RopeArgs(x=A, out=A, token_stride=128, head_stride=64, positions=A, table=A, table_rows=10, tokens=3,
+                         dtype=2, heads=2, head_dim=64, rot_dim=64)
+    refused("rg_rope", INVALID, "null", C.byref(a), None, None)
+    refused("rg_rope", INVALID, "null", None, A, None)
 
 
 def cache(**change):
@@ -156,6 +172,18 @@ def test_attention_head_dims(dim):
 def test_attention_needs_aligned_cache_strides_and_error_words():
     refused("rg_attention_paged", INVALID, "multiples", C.byref(cache(token_stride=129)), C.byref(attention()), A, A, None)
     refused("rg_attention_paged", INVALID, "null", C.byref(cache()), C.byref(attention()), A, None, None)
+
+
+def test_packed_arguments_match_the_structs():
+    """serving.py packs the argument structs itself: the same size and layout as in C."""
+    from rustgears_b200 import serving as sv
+    for pack, struct in ((sv._LINEAR, _native.LinearTokenArgs), (sv._ROPE, _native.RopeArgs),
+                         (sv._CACHE, _native.KvCacheC), (sv._APPEND, _native.KvAppendArgs),
+                         (sv._ATTENTION, _native.PagedAttentionArgs)):
+        fields = struct._fields_
+        got = struct.from_buffer_copy(pack.pack(*range(1, len(fields) + 1)).ljust(C.sizeof(struct), b"\0"))
+        assert [getattr(got, f) for f, _ in fields] == list(range(1, len(fields) + 1))
+        assert pack.size <= C.sizeof(struct) < pack.size + 8
 
 
 def test_python_layer_refuses_before_the_library():
