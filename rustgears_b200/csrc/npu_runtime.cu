@@ -54,6 +54,11 @@ rg_status set_last_error(rg_status st, const char* msg) {
   return st;
 }
 
+void tc_wait_hook(uint64_t* wait_ns, int32_t* starve) {
+  *wait_ns = g_tc_wait_ns.load();
+  *starve = g_tc_starve.load();
+}
+
 #define RG_CUDA_TRY(expr)                                                                   \
   do {                                                                                      \
     cudaError_t e_ = (expr);                                                                \

@@ -94,6 +94,9 @@ struct TokenGemmArgs {
   void* out = nullptr;
   int32_t out_dtype = 0;
   int32_t* err = nullptr;
+  uint64_t wait_ns = 0;  // limit of every pipeline wait (0: the default)
+  int32_t after_quantizer = 0;  // a and a_scale come from the quantizer launched just before
+  int32_t starve = 0;    // test hook: issue no operand loads, so the waits run out
 };
 rg_status launch_gemm_token(const TokenGemmArgs& a, cudaStream_t st);
 

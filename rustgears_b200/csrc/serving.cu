@@ -28,6 +28,7 @@ rg_status refuse(rg_status st, const char* fmt, ...) {
 // The launch's own error, if any; an error that was pending before belongs to someone else
 // and is reported as such by the first call that meets it.
 rg_status launched(const char* what, rg_status st) {
+  if (st == RG_ERR_CUDA) return refuse(st, "%s: TMA descriptor encoding failed", what);
   if (st != RG_OK) return refuse(st, "%s: the sizes exceed the launch limits", what);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? RG_OK : refuse(RG_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
@@ -122,6 +123,7 @@ rg_status rg_gemm_i8_token(const int8_t* a, const float* a_scale, const int8_t* 
   g.a = a; g.a_scale = a_scale; g.w = w; g.w_scale = w_scale; g.bias = bias;
   g.m = m; g.n = n; g.ld = ld; g.ldo = ldo; g.act = act; g.act_param = act_param;
   g.out = out; g.out_dtype = out_dtype; g.err = error_words;
+  tc_wait_hook(&g.wait_ns, &g.starve);
   return launched(f, launch_gemm_token(g, (cudaStream_t)stream));
 }
 
@@ -145,7 +147,8 @@ rg_status rg_linear_i8_token(const rg_linear_token_args* p, void* workspace, int
   TokenGemmArgs g;
   g.a = q; g.a_scale = scale; g.w = p->w; g.w_scale = p->w_scale; g.bias = p->bias;
   g.m = p->m; g.n = p->n; g.ld = p->ld; g.ldo = p->ldo; g.act = p->act; g.act_param = p->act_param;
-  g.out = p->out; g.out_dtype = p->out_dtype; g.err = error_words;
+  g.out = p->out; g.out_dtype = p->out_dtype; g.err = error_words; g.after_quantizer = 1;
+  tc_wait_hook(&g.wait_ns, &g.starve);
   return launched(f, launch_gemm_token(g, (cudaStream_t)stream));
 }
 
