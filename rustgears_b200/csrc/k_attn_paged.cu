@@ -19,10 +19,11 @@
 // second launch and no workspace, and the same order of additions in every run.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <climits>
 
+#include "rg_attn.h"
 #include "rg_mma16.cuh"
-#include "rg_serving.h"
 
 namespace rg {
 namespace {
@@ -33,26 +34,9 @@ using namespace mma16;
 constexpr int kStages = 3;
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// n / d for 0 <= n < 2^31 by multiplication (Granlund and Montgomery, PLDI 1994):
-// m = floor(2^32 (2^l - d) / d) + 1, l = ceil(log2 d).
-struct FastDiv {
-  uint32_t d, m, s;
-  explicit FastDiv(uint32_t v = 1) : d(v) {
-    uint32_t l = 0;
-    while ((1ull << l) < v) ++l;
-    m = (uint32_t)(((1ull << 32) * ((1ull << l) - v)) / v + 1);
-    s = l;
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
-    return (uint32_t)(((uint64_t)__umulhi(n, m) + n) >> s);
-  }
-};
-
 struct Params {
-  PagedAttnArgs p;
-  FastDiv page, group;
+  AttnParams a;
   int32_t splits, tiles;  // blocks over a sequence's keys, and over its rows
-  float scale2;           // scale * log2(e)
 };
 
 template <int D, int WR, int WK>
@@ -77,13 +61,13 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
   using S = Shape<D, WR, WK>;
   constexpr int KT = S::KT;
   extern __shared__ __align__(16) uint8_t smem[];
-  const rg_kv_cache& c = P.p.c;
-  const rg_paged_attention_args& a = P.p.a;
+  const rg_kv_cache& c = P.a.p.c;
+  const rg_paged_attention_args& a = P.a.p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp % WR, wk = warp / WR;
   const int split = blockIdx.x % P.splits, tile = blockIdx.x / P.splits;
   const int hk = blockIdx.y, b = blockIdx.z;
-  const int group = P.group.d;
+  const int group = P.a.group.d;
 
   uint8_t* sq = smem;
   uint8_t* ring = smem + S::kQ;
@@ -93,13 +77,13 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int kv = a.kv_len[b];
   if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) {
-    if (tid == 0) P.p.err[1] = 1;
+    if (tid == 0) P.a.p.err[1] = 1;
     return;
   }
   const int ql = (int)(q1 - q0), rows = ql * group, row0 = tile * S::kRows;
-  if (row0 >= rows) return;
+  if (row0 >= rows || rows <= P.a.min_rows || rows > P.a.max_rows) return;
   // keys seen by the tile's last row
-  const int last_tok = (int)P.group.div((uint32_t)(min(row0 + S::kRows, rows) - 1));
+  const int last_tok = (int)P.a.group.div((uint32_t)(min(row0 + S::kRows, rows) - 1));
   const int seen = a.causal ? max(0, min(kv, kv - ql + last_tok + 1)) : kv;
   const int n_tiles = (seen + KT - 1) / KT;
   const int per = (n_tiles + P.splits - 1) / P.splits;
@@ -109,7 +93,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
   for (int i = tid; i < S::kRows * (D / 8); i += S::kThreads) {
     const int r = i / (D / 8), ch = i % (D / 8), row = row0 + r;
     const bool ok = row < rows;
-    const int tok = (int)P.group.div((uint32_t)(ok ? row : 0)), h = hk * group + (ok ? row : 0) - tok * group;
+    const int tok = (int)P.a.group.div((uint32_t)(ok ? row : 0)), h = hk * group + (ok ? row : 0) - tok * group;
     cp_async16(saddr(sq + r * S::kPitch + ch * 16),
                static_cast<const T*>(a.q) + (q0 + tok) * a.q_token_stride + h * a.q_head_stride + ch * 8, ok);
   }
@@ -119,10 +103,10 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
   const auto look = [&](int t) -> int64_t {
     const int key = t * KT + tid;
     if (t >= t1 || key >= seen) return -1;
-    const uint32_t pi = P.page.div((uint32_t)key);
+    const uint32_t pi = P.a.page.div((uint32_t)key);
     const int64_t page = a.block_table[(int64_t)b * a.block_table_stride + pi];
     if (page < 0 || page >= c.pages) {
-      P.p.err[1] = 1;
+      P.a.p.err[1] = 1;
       return -1;
     }
     return page * c.page_stride + (int64_t)(key - pi * c.page_size) * c.token_stride + hk * c.head_stride;
@@ -156,7 +140,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = row0 + wr * 16 + g + 8 * i;
-    limit[i] = row >= rows ? 0 : a.causal ? min(kv, kv - ql + (int)P.group.div((uint32_t)row) + 1) : kv;
+    limit[i] = row >= rows ? 0 : a.causal ? min(kv, kv - ql + (int)P.a.group.div((uint32_t)row) + 1) : kv;
   }
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -205,7 +189,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
     for (int j = 0; j < S::kKeys / 8; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float v = s[j][i] * P.scale2;
+        const float v = s[j][i] * P.a.scale2;
         s[j][i] = key0 + j * 8 + (i & 1) < limit[i >> 1] ? v : -INFINITY;
         top[i >> 1] = fmaxf(top[i >> 1], s[j][i]);
       }
@@ -310,7 +294,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
   const auto store = [&](int r, int ch, float (&v)[8], float sum) {
     const int row = row0 + r;
     if (row >= rows) return;
-    const int tok = (int)P.group.div((uint32_t)row), h = hk * group + row - tok * group;
+    const int tok = (int)P.a.group.div((uint32_t)row), h = hk * group + row - tok * group;
     const float inv = 1.0f / sum;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = sum == 0.0f ? 0.0f : v[i] * inv;  // no key: zeros
@@ -349,7 +333,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
 }
 
 template <typename T, int D, int WR, int WK>
-rg_status go(const PagedAttnArgs& p, cudaStream_t st) {
+rg_status go(const AttnParams& A, cudaStream_t st) {
   using S = Shape<D, WR, WK>;
   const auto kernel = k_attn_few<T, D, WR, WK>;
   static DeviceOnce once;
@@ -357,14 +341,13 @@ rg_status go(const PagedAttnArgs& p, cudaStream_t st) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   });
+  const PagedAttnArgs& p = A.p;
   Params P;
-  P.p = p;
-  P.page = FastDiv((uint32_t)p.c.page_size);
-  P.group = FastDiv((uint32_t)(p.a.heads / p.c.kv_heads));
-  P.scale2 = p.a.scale * kLog2e;
-  const int64_t rows = (int64_t)p.a.max_q_len * P.group.d;
-  const int64_t tiles = (rows + S::kRows - 1) / S::kRows;
+  P.a = A;
+  int64_t rows = (int64_t)p.a.max_q_len * A.group.d;
   if (rows > INT_MAX || p.c.kv_heads > 65535) return RG_ERR_UNSUPPORTED;
+  rows = std::min<int64_t>(rows, A.max_rows);
+  const int64_t tiles = (rows + S::kRows - 1) / S::kRows;
   // Splits: enough blocks to fill two per SM four times over (unequal lengths even out), while
   // every split keeps two tiles.
   const int64_t blocks = tiles * p.c.kv_heads * p.a.batch;
@@ -389,27 +372,51 @@ rg_status go(const PagedAttnArgs& p, cudaStream_t st) {
 }
 
 template <typename T, int D>
-rg_status go_rows(const PagedAttnArgs& p, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.a.max_q_len * (p.a.heads / p.c.kv_heads);
-  return rows <= 16 ? go<T, D, 1, (D <= 128 ? 4 : 2)>(p, st) : go<T, D, 4, 2>(p, st);
+rg_status go_rows(const AttnParams& A, cudaStream_t st) {
+  const int64_t rows = std::min<int64_t>((int64_t)A.p.a.max_q_len * A.group.d, A.max_rows);
+  return rows <= 16 ? go<T, D, 1, (D <= 128 ? 4 : 2)>(A, st) : go<T, D, 4, 2>(A, st);
 }
 
 template <typename T>
-rg_status go_dim(const PagedAttnArgs& p, cudaStream_t st) {
-  switch (p.c.head_dim) {
-    case 64: return go_rows<T, 64>(p, st);
-    case 96: return go_rows<T, 96>(p, st);
-    case 128: return go_rows<T, 128>(p, st);
-    default: return go_rows<T, 256>(p, st);
+rg_status go_dim(const AttnParams& A, cudaStream_t st) {
+  switch (A.p.c.head_dim) {
+    case 64: return go_rows<T, 64>(A, st);
+    case 96: return go_rows<T, 96>(A, st);
+    case 128: return go_rows<T, 128>(A, st);
+    default: return go_rows<T, 256>(A, st);
   }
 }
+
+rg_status launch_few(const AttnParams& A, cudaStream_t st) {
+  return A.p.c.dtype == RG_DTYPE_F16 ? go_dim<__half>(A, st) : go_dim<__nv_bfloat16>(A, st);
+}
+
+constexpr int kFewRows = 64;
 
 }  // namespace
 
 int64_t attention_paged_workspace(const PagedAttnArgs&) { return 0; }
 
 rg_status launch_attention_paged(const PagedAttnArgs& p, cudaStream_t st) {
-  return p.c.dtype == RG_DTYPE_F16 ? go_dim<__half>(p, st) : go_dim<__nv_bfloat16>(p, st);
+  AttnParams A;
+  A.p = p;
+  A.page = FastDiv((uint32_t)p.c.page_size);
+  A.group = FastDiv((uint32_t)(p.a.heads / p.c.kv_heads));
+  A.scale2 = p.a.scale * kLog2e;
+  A.min_rows = 0;
+  A.max_rows = INT_MAX;
+  const int64_t rows = (int64_t)p.a.max_q_len * A.group.d;
+  if (rows <= kFewRows || !attention_tc_takes(p)) return launch_few(A, st);
+  // Chunks go to the tensor-core kernel.  Where the batch may hold shorter sequences too (the
+  // tokens are fewer than batch times the longest), those take the kernel for few rows.
+  if (p.a.batch > 1 && p.a.tokens < (int64_t)p.a.batch * p.a.max_q_len) {
+    A.max_rows = kFewRows;
+    const rg_status s = launch_few(A, st);
+    if (s != RG_OK) return s;
+    A.min_rows = kFewRows;
+    A.max_rows = INT_MAX;
+  }
+  return launch_attention_tc(A, st);
 }
 
 }  // namespace rg

@@ -125,6 +125,8 @@ struct PagedAttnArgs {
   rg_paged_attention_args a;
   void* workspace = nullptr;
   int32_t* err = nullptr;
+  uint64_t wait_ns = 0;  // as TokenGemmArgs
+  int32_t starve = 0;
 };
 int64_t attention_paged_workspace(const PagedAttnArgs& a);
 rg_status launch_attention_paged(const PagedAttnArgs& a, cudaStream_t st);

@@ -279,6 +279,7 @@ rg_status rg_attention_paged(const rg_kv_cache* cache, const rg_paged_attention_
   p.a = *args;
   p.workspace = workspace;
   p.err = error_words;
+  tc_wait_hook(&p.wait_ns, &p.starve);
   const int64_t need = attention_paged_workspace(p);
   if (need > 0 && (!workspace || !aligned(workspace, 256)))
     return refuse(RG_ERR_INVALID_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed", f, (long long)need);

@@ -619,6 +619,31 @@ def test_linear_bounded_waits_are_reported(gpu, sv, m):
     same(torch, got, rounded(torch, linear_reference(x, wq, sw, b, 0), "f32"))
 
 
+def test_attention_bounded_waits_are_reported(gpu, sv):
+    """Without loads the chunk kernel's waits run out: reported, and the next call is right."""
+    torch, L = gpu, _native.lib()
+    args = make_batch(torch, [(100, 300)], 4, 2, 64, torch.float16, 16, "token")
+    try:
+        L.rg_debug_set_tc_wait(1000000, 1)
+        sv.attention_paged(*args, max_q_len=100, max_kv_len=300)
+        with pytest.raises(_native.RgError, match="bounded wait") as e:
+            sv.check()
+        assert e.value.status == _native.RG_ERR_TIMEOUT
+    finally:
+        L.rg_debug_set_tc_wait(0, 0)
+    check_attention(torch, sv, [(100, 300)], 4, 2, 64, torch.float16, 16, "token")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 384])
+def test_attention_long_chunks(gpu, sv, dim, page):
+    """Several tiles of rows and keys, pages of every size the tensor-core kernel takes."""
+    for lens, heads, kv_heads in (([(700, 2100), (90, 640), (1, 1500)], 6, 2), ([(333, 333), (257, 1024)], 3, 3),
+                                  ([(60, 4000)], 16, 2)):
+        check_attention(gpu, sv, lens, heads, kv_heads, dim, gpu.bfloat16, page, "head" if page < 64 else "token",
+                        seed=page)
+
+
 def test_zero_sizes(gpu, sv):
     torch = gpu
     w, ws = sv.quantize_weight_i8(torch.randn(8, 32, device="cuda"))
