@@ -187,6 +187,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // S_g (and P_g over its first 64 columns) at 128 g, O_g at 256 + D g
 
+  // A softmax thread holds its row's 128 scores.  The launch gives 384 x 168 = 64512 registers;
+  // 128 x 56 + 256 x 224 is the same sum.
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0) {
     // ---------------- loads ----------------
     const int per_tile = p.page_log2 >= 0 ? kTile >> p.page_log2 : 1;  // pages of a tile
@@ -310,7 +314,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(v_fixed);
       }
     }
-  } else if (warp >= 4 && (warp - 4) / 4 < groups) {
+  }
+  } else {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+  if ((warp - 4) / 4 < groups) {
     // ---------------- softmax ----------------
     const int g = (warp - 4) / 4;
     const int tr = (warp & 3) * 32 + lane;  // row of the group, and its TMEM lane
@@ -428,6 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     tc_fence_before();
+  }
   }
 
   __syncwarp();
