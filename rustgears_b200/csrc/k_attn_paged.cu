@@ -13,12 +13,12 @@
 //
 // Bound: memory for few rows (keys and values are read once: 4 head_dim bytes per key and
 // key head; 16 rows fill one m16n8k16 fragment, whose rate is far above what the loads
-// need).  A three-stage ring of cp.async tiles keeps two tiles in flight per block.
-// Few (sequence, head) pairs leave SMs idle, so a sequence's keys are split over a cluster
-// of up to 16 blocks that join their partial rows through distributed shared memory: no
-// second launch and no workspace, and the same order of additions in every run.
-#include <cooperative_groups.h>
-
+// need).  A three-stage ring of cp.async tiles keeps two tiles in flight per block, two blocks
+// per SM.  Few (sequence, head) pairs leave SMs idle, so a sequence's keys are split over
+// blocks whose partial rows a second, overlapped launch joins in a fixed order.  (A cluster
+// of up to 16 blocks joining through distributed shared memory was slower: the blocks of a
+// cluster start together, which costs a wait for 16 free places; 16.2 against 9 us at one
+// token over 4001 keys.)
 #include <algorithm>
 #include <climits>
 
@@ -28,16 +28,10 @@
 namespace rg {
 namespace {
 
-namespace cg = cooperative_groups;
 using namespace mma16;
 
 constexpr int kStages = 3;
 constexpr float kLog2e = 1.44269504088896340736f;
-
-struct Params {
-  AttnParams a;
-  int32_t splits, tiles;  // blocks over a sequence's keys, and over its rows
-};
 
 template <int D, int WR, int WK>
 struct Shape {
@@ -57,59 +51,63 @@ struct Shape {
 };
 
 template <typename T, int D, int WR, int WK>
-__global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
+__global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const AttnParams P) {
   using S = Shape<D, WR, WK>;
   constexpr int KT = S::KT;
   extern __shared__ __align__(16) uint8_t smem[];
-  const rg_kv_cache& c = P.a.p.c;
-  const rg_paged_attention_args& a = P.a.p.a;
+  const rg_kv_cache& c = P.p.c;
+  const rg_paged_attention_args& a = P.p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp % WR, wk = warp / WR;
   const int split = blockIdx.x % P.splits, tile = blockIdx.x / P.splits;
   const int hk = blockIdx.y, b = blockIdx.z;
-  const int group = P.a.group.d;
+  const int group = P.group.d;
 
   uint8_t* sq = smem;
   uint8_t* ring = smem + S::kQ;
   int64_t* offs = reinterpret_cast<int64_t*>(ring + kStages * S::kStage);  // [kStages + 1][KT], -1: zeros
 
-  // The same for every block of a cluster, so that all of them leave or stay together.
+  grid_launch_dependents();
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int kv = a.kv_len[b];
   if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) {
-    if (tid == 0) P.a.p.err[1] = 1;
+    if (tid == 0) P.p.err[1] = 1;
     return;
   }
   const int ql = (int)(q1 - q0), rows = ql * group, row0 = tile * S::kRows;
-  if (row0 >= rows || rows <= P.a.min_rows || rows > P.a.max_rows) return;
+  if (row0 >= rows || rows <= P.min_rows || rows > P.max_rows) return;
   // keys seen by the tile's last row
-  const int last_tok = (int)P.a.group.div((uint32_t)(min(row0 + S::kRows, rows) - 1));
+  const int last_tok = (int)P.group.div((uint32_t)(min(row0 + S::kRows, rows) - 1));
   const int seen = a.causal ? max(0, min(kv, kv - ql + last_tok + 1)) : kv;
-  const int n_tiles = (seen + KT - 1) / KT;
-  const int per = (n_tiles + P.splits - 1) / P.splits;
-  const int t0 = min(split * per, n_tiles), t1 = min(t0 + per, n_tiles);
+  const KeySplit ks(seen, KT, P.splits);
+  if (split >= ks.active) return;
+  const int t0 = split * ks.per, t1 = min(t0 + ks.per, ks.tiles);
 
   // ---- queries: rows past the last one are zeros ----
   for (int i = tid; i < S::kRows * (D / 8); i += S::kThreads) {
     const int r = i / (D / 8), ch = i % (D / 8), row = row0 + r;
     const bool ok = row < rows;
-    const int tok = (int)P.a.group.div((uint32_t)(ok ? row : 0)), h = hk * group + (ok ? row : 0) - tok * group;
+    const int tok = (int)P.group.div((uint32_t)(ok ? row : 0)), h = hk * group + (ok ? row : 0) - tok * group;
     cp_async16(saddr(sq + r * S::kPitch + ch * 16),
                static_cast<const T*>(a.q) + (q0 + tok) * a.q_token_stride + h * a.q_head_stride + ch * 8, ok);
   }
   cp_async_commit();
 
   // ---- key addresses: thread r < KT looks tile t's key r up, one tile ahead of its loads ----
-  const auto look = [&](int t) -> int64_t {
+  const int32_t* table = a.block_table + (int64_t)b * a.block_table_stride;
+  constexpr int kNone = INT_MIN;  // no such key
+  const auto look = [&](int t) -> int {
     const int key = t * KT + tid;
-    if (t >= t1 || key >= seen) return -1;
-    const uint32_t pi = P.a.page.div((uint32_t)key);
-    const int64_t page = a.block_table[(int64_t)b * a.block_table_stride + pi];
+    return tid < KT && t < t1 && key < seen ? table[P.page.div((uint32_t)key)] : kNone;
+  };
+  const auto offset = [&](int t, int page) -> int64_t {
     if (page < 0 || page >= c.pages) {
-      P.a.p.err[1] = 1;
+      if (page != kNone) P.p.err[1] = 1;
       return -1;
     }
-    return page * c.page_stride + (int64_t)(key - pi * c.page_size) * c.token_stride + hk * c.head_stride;
+    const int key = t * KT + tid;
+    return page * c.page_stride + (int64_t)(key - P.page.div((uint32_t)key) * c.page_size) * c.token_stride +
+           hk * c.head_stride;
   };
   const auto load = [&](int t) {  // tile t into its stage
     const int stage = (t - t0) % kStages;
@@ -125,14 +123,21 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
       cp_async16(base + S::kTile + r * S::kPitch + ch * 16, static_cast<const T*>(c.v) + at, ok);
     }
   };
-  if (tid < KT)
-    for (int s = 0; s < kStages; ++s) offs[s * KT + tid] = look(t0 + s);
+  int ahead;
+  {
+    int page[kStages];
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) page[s] = look(t0 + s);
+    ahead = look(t0 + kStages);
+    if (tid < KT)
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) offs[s * KT + tid] = offset(t0 + s, page[s]);
+  }
   __syncthreads();
   for (int s = 0; s < kStages - 1; ++s) {
     if (t0 + s < t1) load(t0 + s);
     cp_async_commit();
   }
-  int64_t ahead = tid < KT ? look(t0 + kStages) : -1;
 
   // ---- main loop ----
   const int g = lane >> 2, t4 = lane & 3;
@@ -140,7 +145,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = row0 + wr * 16 + g + 8 * i;
-    limit[i] = row >= rows ? 0 : a.causal ? min(kv, kv - ql + (int)P.a.group.div((uint32_t)row) + 1) : kv;
+    limit[i] = row >= rows ? 0 : a.causal ? min(kv, kv - ql + (int)P.group.div((uint32_t)row) + 1) : kv;
   }
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -153,7 +158,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
   for (int t = t0; t < t1; ++t) {
     cp_async_wait<kStages - 2>();
     if (tid < KT) {
-      offs[((t - t0 + kStages) % (kStages + 1)) * KT + tid] = ahead;
+      offs[((t - t0 + kStages) % (kStages + 1)) * KT + tid] = offset(t + kStages, ahead);
       ahead = look(t + kStages + 1);
     }
     __syncthreads();  // tile t has landed, and everyone is done with tile t - 1's stage
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
     for (int j = 0; j < S::kKeys / 8; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float v = s[j][i] * P.a.scale2;
+        const float v = s[j][i] * P.scale2;
         s[j][i] = key0 + j * 8 + (i & 1) < limit[i >> 1] ? v : -INFINITY;
         top[i >> 1] = fmaxf(top[i >> 1], s[j][i]);
       }
@@ -290,46 +295,94 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const Params P) {
       fl[r0 + 8 * i] = L[i];
     }
 
-  // ---- join the splits, normalise, store: block `split` of the cluster takes a share ----
-  const auto store = [&](int r, int ch, float (&v)[8], float sum) {
-    const int row = row0 + r;
-    if (row >= rows) return;
-    const int tok = (int)P.a.group.div((uint32_t)row), h = hk * group + row - tok * group;
-    const float inv = 1.0f / sum;
+  // ---- store: the rows, or what this split has of them ----
+  __syncthreads();
+  const int64_t part = (int64_t)split * a.tokens * a.heads;
+  for (int i = tid; i < S::kRows * (D / 8); i += S::kThreads) {
+    const int r = i / (D / 8), ch = i % (D / 8), row = row0 + r;
+    if (row >= rows) break;
+    const int tok = (int)P.group.div((uint32_t)row), h = hk * group + row - tok * group;
+    float v[8];
+    Pack<float, 8>::load(jo + r * S::kOPitch + ch * 8, v);
+    if (ks.active > 1) {
+      const int64_t at = part + (q0 + tok) * a.heads + h;
+      Pack<float, 8>::store(P.part_o + at * D + ch * 8, v);
+      if (ch == 0) P.part_ml[at] = make_float2(fm[r], fl[r]);
+    } else {
+      const float inv = 1.0f / fl[r];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = sum == 0.0f ? 0.0f : v[i] * inv;  // no key: zeros
-    Pack<T, 8>::store(static_cast<T*>(a.out) + (q0 + tok) * a.out_token_stride + h * a.out_head_stride + ch * 8, v);
-  };
-  if (P.splits == 1) {
+      for (int x = 0; x < 8; ++x) v[x] = fl[r] == 0.0f ? 0.0f : v[x] * inv;  // no key: zeros
+      Pack<T, 8>::store(static_cast<T*>(a.out) + (q0 + tok) * a.out_token_stride + h * a.out_head_stride + ch * 8, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the splits' partial rows, in a fixed order: W of a block's 8 warps per row, each adding
+// every W-th split (few rows and many splits are a matter of latency: their loads are all in
+// flight at once).  Launched beside the end of the kernels before it (its blocks wait for them).
+// ---------------------------------------------------------------------------
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(256) k_attn_join(const JoinParams J) {
+  const AttnParams& P = J.A;
+  const rg_paged_attention_args& a = P.p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hk = blockIdx.y, b = blockIdx.z, group = P.group.d;
+  const int row = blockIdx.x * (8 / W) + warp / W, w = warp % W;
+  const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
+  const int kv = a.kv_len[b];
+  grid_dependency_wait();
+  if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) return;
+  const int ql = (int)(q1 - q0), rows = ql * group;
+  if (row >= rows) return;
+  const TileShape& sh = rows <= J.limit ? J.few : J.many;
+  const int last = min(row / sh.rows * sh.rows + sh.rows, rows) - 1;  // of the row's tile
+  const int seen = a.causal ? max(0, min(kv, kv - ql + (int)P.group.div((uint32_t)last) + 1)) : kv;
+  const KeySplit ks(seen, sh.keys, sh.splits);
+  if (ks.active == 1) return;  // stored by its block
+  const int tok = (int)P.group.div((uint32_t)row), h = hk * group + row - tok * group;
+  const int64_t at = (q0 + tok) * a.heads + h, step = a.tokens * a.heads;
+  float top = -INFINITY;
+  for (int s = lane; s < ks.active; s += 32) top = fmaxf(top, P.part_ml[at + s * step].x);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  const float base = top == -INFINITY ? 0.0f : top;
+  constexpr int N = D / 32;  // dimensions N lane .. + N - 1
+  float v[N], sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.0f;
+#pragma unroll 4
+  for (int s = w; s < ks.active; s += W) {
+    const float2 ml = P.part_ml[at + s * step];
+    float o[N];
+    const float* src = P.part_o + (at + s * step) * D + lane * N;
+    if constexpr (N % 2 == 0) {
+      Pack<float, N>::load(src, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = src[i];
+    }
+    const float e = ex2(ml.x - base);
+    sum += e * ml.y;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += e * o[i];
+  }
+  if constexpr (W > 1) {
+    __shared__ float add[8][33 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) add[warp][lane * N + i] = v[i];
+    if (lane == 0) add[warp][32 * N] = sum;
     __syncthreads();
-    for (int i = tid; i < S::kRows * (D / 8); i += S::kThreads) {
-      const int r = i / (D / 8), ch = i % (D / 8);
-      float v[8];
-      Pack<float, 8>::load(jo + r * S::kOPitch + ch * 8, v);
-      store(r, ch, v, fl[r]);
-    }
-    return;
-  }
-  cg::cluster_group cl = cg::this_cluster();
-  cl.sync();
-  for (int i = split * S::kThreads + tid; i < S::kRows * (D / 8); i += P.splits * S::kThreads) {
-    const int r = i / (D / 8), ch = i % (D / 8);
-    float top = -INFINITY, sum = 0.0f, v[8];
-    for (int w = 0; w < P.splits; ++w) top = fmaxf(top, cl.map_shared_rank(fm, w)[r]);
-    const float base = top == -INFINITY ? 0.0f : top;
+    if (w != 0) return;
+    for (int x = 1; x < W; ++x) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    for (int w = 0; w < P.splits; ++w) {
-      const float e = ex2(cl.map_shared_rank(fm, w)[r] - base);
-      sum += e * cl.map_shared_rank(fl, w)[r];
-      float x[8];
-      Pack<float, 8>::load(cl.map_shared_rank(jo, w) + r * S::kOPitch + ch * 8, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += e * x[j];
+      for (int i = 0; i < N; ++i) v[i] += add[warp + x][lane * N + i];
+      sum += add[warp + x][32 * N];
     }
-    store(r, ch, v, sum);
   }
-  cl.sync();  // no block leaves while another reads its shared memory
+  const float inv = 1.0f / sum;
+  T* dst = static_cast<T*>(a.out) + (q0 + tok) * a.out_token_stride + h * a.out_head_stride + lane * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) dst[i] = ElemOf<T>::from(sum == 0.0f ? 0.0f : v[i] * inv);
 }
 
 template <typename T, int D, int WR, int WK>
@@ -337,44 +390,22 @@ rg_status go(const AttnParams& A, cudaStream_t st) {
   using S = Shape<D, WR, WK>;
   const auto kernel = k_attn_few<T, D, WR, WK>;
   static DeviceOnce once;
-  once.run([&] {  // a failure shows in the launch
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  });
-  const PagedAttnArgs& p = A.p;
-  Params P;
-  P.a = A;
-  int64_t rows = (int64_t)p.a.max_q_len * A.group.d;
-  if (rows > INT_MAX || p.c.kv_heads > 65535) return RG_ERR_UNSUPPORTED;
-  rows = std::min<int64_t>(rows, A.max_rows);
+  once.run([&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); });
+  const int64_t rows = std::min<int64_t>((int64_t)A.p.a.max_q_len * A.group.d, A.max_rows);
   const int64_t tiles = (rows + S::kRows - 1) / S::kRows;
-  // Splits: enough blocks to fill two per SM four times over (unequal lengths even out), while
-  // every split keeps two tiles.
-  const int64_t blocks = tiles * p.c.kv_heads * p.a.batch;
-  int splits = 1;
-  while (splits < 16 && blocks * splits < 148 * 8 && (int64_t)splits * 2 * 2 * S::KT <= p.a.max_kv_len) splits *= 2;
-  if (tiles * splits > INT_MAX) return RG_ERR_UNSUPPORTED;
-  P.splits = splits;
-  P.tiles = (int32_t)tiles;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * splits), (unsigned)p.c.kv_heads, (unsigned)p.a.batch);
-  cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, P);
+  if (tiles * A.splits > INT_MAX) return RG_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)(tiles * A.splits), (unsigned)A.p.c.kv_heads, (unsigned)A.p.a.batch);
+  kernel<<<grid, S::kThreads, S::kSmem, st>>>(A);
   return RG_OK;
 }
 
+// Rows of a block: 16 (one fragment, all warps on the keys) or 64.
+inline int few_rows(const AttnParams& A) {
+  return std::min<int64_t>((int64_t)A.p.a.max_q_len * A.group.d, A.max_rows) <= 16 ? 16 : 64;
+}
 template <typename T, int D>
 rg_status go_rows(const AttnParams& A, cudaStream_t st) {
-  const int64_t rows = std::min<int64_t>((int64_t)A.p.a.max_q_len * A.group.d, A.max_rows);
-  return rows <= 16 ? go<T, D, 1, (D <= 128 ? 4 : 2)>(A, st) : go<T, D, 4, 2>(A, st);
+  return few_rows(A) == 16 ? go<T, D, 1, (D <= 128 ? 4 : 2)>(A, st) : go<T, D, 4, 2>(A, st);
 }
 
 template <typename T>
@@ -391,32 +422,134 @@ rg_status launch_few(const AttnParams& A, cudaStream_t st) {
   return A.p.c.dtype == RG_DTYPE_F16 ? go_dim<__half>(A, st) : go_dim<__nv_bfloat16>(A, st);
 }
 
+template <typename T, int W>
+void launch_join(const JoinParams& J, int64_t rows, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((rows * W + 7) / 8), (unsigned)J.A.p.c.kv_heads, (unsigned)J.A.p.a.batch);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  switch (J.A.p.c.head_dim) {
+    case 64: cudaLaunchKernelEx(&cfg, k_attn_join<T, 64, W>, J); break;
+    case 96: cudaLaunchKernelEx(&cfg, k_attn_join<T, 96, W>, J); break;
+    case 128: cudaLaunchKernelEx(&cfg, k_attn_join<T, 128, W>, J); break;
+    default: cudaLaunchKernelEx(&cfg, k_attn_join<T, 256, W>, J); break;
+  }
+}
+template <typename T>
+void launch_join(const JoinParams& J, int64_t rows, cudaStream_t st) {
+  // a block per row where the rows do not fill the SMs by themselves
+  if (rows * J.A.p.c.kv_heads * J.A.p.a.batch <= 148 * 8 && std::max(J.few.splits, J.many.splits) > 4)
+    launch_join<T, 8>(J, rows, st);
+  else launch_join<T, 1>(J, rows, st);
+}
+
+// Splits of a launch of `blocks` blocks over `tiles` key tiles each, `slots` blocks running at
+// once: the least of rounds x (a block's start + its tiles) + the join, in microseconds; the
+// times were measured (a start of about 3, a join of about 2 and of 8 bytes a partial value at
+// 5 TB/s).
+int split_keys(int64_t blocks, int64_t tiles, int slots, double tile_us, int min_tiles, double join_us) {
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 64 && (s == 1 || tiles >= (int64_t)s * min_tiles); ++s) {
+    const double t = (double)((blocks * s + slots - 1) / slots) * (3.0 + tile_us * (double)((tiles + s - 1) / s)) +
+                     (s > 1 ? 2.0 + s * join_us : 0.0);
+    if (t < 0.97 * least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// Up to so many rows (tokens times the heads that share a key head) a sequence takes the kernel
+// for few rows.
 constexpr int kFewRows = 64;
 
-}  // namespace
-
-int64_t attention_paged_workspace(const PagedAttnArgs&) { return 0; }
-
-rg_status launch_attention_paged(const PagedAttnArgs& p, cudaStream_t st) {
+struct Plan {
   AttnParams A;
+  bool few, many;
+  TileShape few_shape, many_shape;
+  int64_t rows;
+  int64_t part_rows;  // rows of partial results, all splits
+};
+
+rg_status make_plan(const PagedAttnArgs& p, Plan& L) {
+  AttnParams& A = L.A;
   A.p = p;
   A.page = FastDiv((uint32_t)p.c.page_size);
   A.group = FastDiv((uint32_t)(p.a.heads / p.c.kv_heads));
   A.scale2 = p.a.scale * kLog2e;
-  A.min_rows = 0;
-  A.max_rows = INT_MAX;
-  const int64_t rows = (int64_t)p.a.max_q_len * A.group.d;
-  if (rows <= kFewRows || !attention_tc_takes(p)) return launch_few(A, st);
+  A.splits = 1;
+  A.part_o = nullptr;
+  A.part_ml = nullptr;
+  L.rows = (int64_t)p.a.max_q_len * A.group.d;
+  if (L.rows > INT_MAX || p.c.kv_heads > 65535) return RG_ERR_UNSUPPORTED;
   // Chunks go to the tensor-core kernel.  Where the batch may hold shorter sequences too (the
   // tokens are fewer than batch times the longest), those take the kernel for few rows.
-  if (p.a.batch > 1 && p.a.tokens < (int64_t)p.a.batch * p.a.max_q_len) {
-    A.max_rows = kFewRows;
-    const rg_status s = launch_few(A, st);
-    if (s != RG_OK) return s;
-    A.min_rows = kFewRows;
-    A.max_rows = INT_MAX;
+  L.many = L.rows > kFewRows && attention_tc_takes(p);
+  L.few = !L.many || (p.a.batch > 1 && p.a.tokens < (int64_t)p.a.batch * p.a.max_q_len);
+  A.min_rows = 0;
+  A.max_rows = L.many ? kFewRows : INT_MAX;
+  const int d = p.c.head_dim;
+  const double row_us = 8.0 * d * (double)p.a.tokens * p.a.heads / 5e6;  // partial rows written and read
+  const int64_t seqs = (int64_t)p.c.kv_heads * p.a.batch;
+  L.few_shape = {few_rows(A), d <= 128 ? 64 : 32, 1};
+  L.many_shape = {kTcRows, kTcKeys, 1};
+  if (L.few) {
+    const int64_t tiles = (std::min<int64_t>(L.rows, A.max_rows) + L.few_shape.rows - 1) / L.few_shape.rows;
+    L.few_shape.splits = split_keys(seqs * tiles, (p.a.max_kv_len + L.few_shape.keys - 1) / L.few_shape.keys, 296,
+                                    d <= 64 ? 0.4 : 0.8, 2, row_us);
   }
-  return launch_attention_tc(A, st);
+  if (L.many)
+    L.many_shape.splits = split_keys(seqs * ((L.rows + kTcRows - 1) / kTcRows),
+                                     (p.a.max_kv_len + kTcKeys - 1) / kTcKeys, 148, 2.3, 2, row_us);
+  const int most = std::max(L.few ? L.few_shape.splits : 1, L.many ? L.many_shape.splits : 1);
+  L.part_rows = most > 1 ? most * p.a.tokens * p.a.heads : 0;
+  return RG_OK;
+}
+
+}  // namespace
+
+int64_t attention_paged_workspace(const PagedAttnArgs& p) {
+  Plan L;
+  if (make_plan(p, L) != RG_OK) return 0;
+  return L.part_rows * (p.c.head_dim * 4 + 8);
+}
+
+rg_status launch_attention_paged(const PagedAttnArgs& p, cudaStream_t st) {
+  Plan L;
+  rg_status s = make_plan(p, L);
+  if (s != RG_OK) return s;
+  AttnParams& A = L.A;
+  A.part_o = static_cast<float*>(p.workspace);
+  A.part_ml = reinterpret_cast<float2*>(A.part_o + L.part_rows * p.c.head_dim);
+  if (L.few) {
+    A.splits = L.few_shape.splits;
+    s = launch_few(A, st);
+    if (s != RG_OK) return s;
+  }
+  if (L.many) {
+    A.splits = L.many_shape.splits;
+    A.min_rows = L.few ? kFewRows : 0;
+    A.max_rows = INT_MAX;
+    s = launch_attention_tc(A, L.few, st);
+    if (s != RG_OK) return s;
+  }
+  if (L.part_rows) {
+    JoinParams J;
+    J.A = A;
+    J.few = L.few_shape;
+    J.many = L.many_shape;
+    J.limit = !L.many ? INT_MAX : L.few ? kFewRows : 0;
+    if (p.c.dtype == RG_DTYPE_F16) launch_join<__half>(J, L.rows, st);
+    else launch_join<__nv_bfloat16>(J, L.rows, st);
+  }
+  return RG_OK;
 }
 
 }  // namespace rg

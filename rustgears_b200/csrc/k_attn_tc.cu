@@ -42,7 +42,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kThreads = 384;
-constexpr int kTile = 128;  // keys of a tile, rows of a group
+constexpr int kTile = kTcKeys;  // keys of a tile, rows of a group
 constexpr uint64_t kWaitNs = 2000000000ull, kDrainNs = 200000000ull;
 constexpr float kLazy = 8.0f;
 
@@ -143,24 +143,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   const rg_paged_attention_args& a = p.P.p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.y, b = blockIdx.z, group = (int)p.P.group.d;
+  grid_launch_dependents();
 
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int kv = a.kv_len[b];
   if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) {
     if (threadIdx.x == 0) p.P.p.err[1] = 1;
+    grid_dependency_wait();
     return;
   }
   const int ql = (int)(q1 - q0), rows = ql * group;
   // the last rows see the most keys: they start first
-  const int row0 = (int)(gridDim.x - 1 - blockIdx.x) * 2 * kTile;
-  if (row0 >= rows || rows <= p.P.min_rows) return;
+  const int turned = (int)(gridDim.x - 1 - blockIdx.x);
+  const int row0 = turned / p.P.splits * 2 * kTile, split = turned % p.P.splits;
+  if (row0 >= rows || rows <= p.P.min_rows) {
+    grid_dependency_wait();
+    return;
+  }
   const int groups = rows - row0 > kTile ? 2 : 1;
   const auto keys_of = [&](int row) {  // keys that a row sees
     return a.causal ? max(0, min(kv, kv - ql + (int)p.P.group.div((uint32_t)row) + 1)) : kv;
   };
   const int seen = keys_of(min(row0 + groups * kTile, rows) - 1);
-  const int tiles = (seen + kTile - 1) / kTile;
-  const bool tail = tiles * kTile > kv;  // the last tile has rows past the last key
+  const KeySplit ks(seen, kTile, p.P.splits);
+  if (split >= ks.active) {
+    grid_dependency_wait();
+    return;
+  }
+  // this split's tiles t0 .. t0 + tiles - 1, called 0 .. tiles - 1 below
+  const int t0 = split * ks.per, tiles = min(t0 + ks.per, ks.tiles) - t0;
+  const bool tail = (t0 + tiles) * kTile > kv;  // the last tile has rows past the last key
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -197,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int32_t* table = a.block_table + (int64_t)b * a.block_table_stride;
     const auto look = [&](int n) -> int {  // lane i: the page of tile n's i-th box
       if (lane >= per_tile || n >= tiles) return 0;
-      const int key = n * kTile + lane * p.box;
+      const int key = (t0 + n) * kTile + lane * p.box;
       if (key >= kv) return 0;
       const int page = table[p.P.page.div((uint32_t)key)];
       if (page >= 0 && page < c.pages) return page;
@@ -210,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int n = 0; n < tiles && ok; ++n) {
       const int page = next;
       next = look(n + 1);
-      const int key0 = n * kTile;
+      const int key0 = (t0 + n) * kTile;
       const int pages = p.page_log2 >= 0 ? min(per_tile, (kv - key0 + p.box - 1) >> p.page_log2) : 1;
       const int tok0 = p.page_log2 >= 0 ? 0 : key0 - (int)p.P.page.div((uint32_t)key0) * c.page_size;
       for (int which = 0; which < 2; ++which, ++op) {
@@ -305,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool ok = mbar_wait(v_here, 0, abort, p.wait_ns);
       if (__all_sync(0xffffffffu, ok)) {
         uint8_t* v = ring + (op % C::kStages) * C::kOperand;
-        const int first = kv - (tiles - 1) * kTile;  // whole rows: the swizzle stays inside a row
+        const int first = kv - (t0 + tiles - 1) * kTile;  // whole rows: the swizzle stays inside a row
         for (int h = 0; h < C::kHalves; ++h)
           for (int i = first * 8 + lane; i < kTile * 8; i += 32)
             *reinterpret_cast<uint4*>(v + h * C::kSub + i * 16) = make_uint4(0, 0, 0, 0);
@@ -355,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) tmem_ld32(ts + i * 32, v[i]);
       tmem_ld_wait();
-      if ((n + 1) * kTile > all_see) {
-        const int left = limit - n * kTile;
+      if ((t0 + n + 1) * kTile > all_see) {
+        const int left = limit - (t0 + n) * kTile;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -416,21 +428,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) *abort = 1;
     T* dst = static_cast<T*>(a.out) + (q0 + tok) * a.out_token_stride + head * a.out_head_stride;
+    const int64_t part = ((int64_t)split * a.tokens + q0 + tok) * a.heads + head;
+    if (ok && real && ks.active > 1) p.P.part_ml[part] = make_float2(m, l);
     const float inv = 1.0f / l;
     if (ok) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         uint32_t o[32];
+        __syncwarp();
         if (tiles > 0) {
           tmem_ld32(to + i * 32, o);
           tmem_ld_wait();
         }
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
+        for (int j = 0; j < 32 && real; j += 8) {
           float y[8];
+          if (ks.active > 1) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = l == 0.0f ? 0.0f : u2f(o[j + k]) * inv;  // no key: zeros
-          if (real) Pack<T, 8>::store(dst + i * 32 + j, y);
+            for (int k = 0; k < 8; ++k) y[k] = u2f(o[j + k]);
+            Pack<float, 8>::store(p.P.part_o + part * D + i * 32 + j, y);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = l == 0.0f ? 0.0f : u2f(o[j + k]) * inv;  // no key: zeros
+            Pack<T, 8>::store(dst + i * 32 + j, y);
+          }
         }
       }
     }
@@ -442,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort) atomicExch(p.P.p.err, 1);
+  grid_dependency_wait();  // when this launch ends, so has the one it ran beside
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -466,7 +488,7 @@ bool cache_map(CUtensorMap* map, void* base, const rg_kv_cache& c, int box) {
 }
 
 template <typename T, int D>
-rg_status go(const AttnParams& P, cudaStream_t st) {
+rg_status go(const AttnParams& P, bool beside, cudaStream_t st) {
   using C = Cfg<D>;
   const auto kernel = k_attn_tc<T, D>;
   static DeviceOnce once;
@@ -485,10 +507,19 @@ rg_status go(const AttnParams& P, cudaStream_t st) {
   p.starve = P.p.starve;
   CUtensorMap mk, mv;
   if (!cache_map<T>(&mk, c.k, c, p.box) || !cache_map<T>(&mv, c.v, c, p.box)) return RG_ERR_CUDA;
-  const int64_t rows = (int64_t)P.p.a.max_q_len * P.group.d, blocks = (rows + 2 * kTile - 1) / (2 * kTile);
-  if (rows > INT_MAX || c.kv_heads > 65535) return RG_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)P.p.a.batch);
-  kernel<<<grid, kThreads, C::kSmem, st>>>(mk, mv, p);
+  const int64_t rows = (int64_t)P.p.a.max_q_len * P.group.d, blocks = (rows + kTcRows - 1) / kTcRows * P.splits;
+  if (blocks > INT_MAX) return RG_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)P.p.a.batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, mk, mv, p);
   return RG_OK;
 }
 
@@ -503,9 +534,9 @@ bool attention_tc_takes(const PagedAttnArgs& p) {
   return p.c.page_stride < most && p.c.token_stride < most && p.c.head_stride < most;
 }
 
-rg_status launch_attention_tc(const AttnParams& P, cudaStream_t st) {
-  if (P.p.c.dtype == RG_DTYPE_F16) return P.p.c.head_dim == 64 ? go<__half, 64>(P, st) : go<__half, 128>(P, st);
-  return P.p.c.head_dim == 64 ? go<__nv_bfloat16, 64>(P, st) : go<__nv_bfloat16, 128>(P, st);
+rg_status launch_attention_tc(const AttnParams& P, bool beside, cudaStream_t st) {
+  if (P.p.c.dtype == RG_DTYPE_F16) return P.p.c.head_dim == 64 ? go<__half, 64>(P, beside, st) : go<__half, 128>(P, beside, st);
+  return P.p.c.head_dim == 64 ? go<__nv_bfloat16, 64>(P, beside, st) : go<__nv_bfloat16, 128>(P, beside, st);
 }
 
 }  // namespace rg
