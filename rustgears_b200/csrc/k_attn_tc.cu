@@ -66,16 +66,6 @@ struct TcParams {
   int32_t starve;
 };
 
-// 4-D tile load (dimension, token, head, page).
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y,
-                                            int32_t z, int32_t w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-      "[%2];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
-
 // Instruction descriptor of tcgen05.mma kind::f16: f32 sums, A and B of one 16-bit type, B
 // K-major or (b_mn) MN-major.
 template <typename T>
@@ -94,20 +84,6 @@ __device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t saddr, uint32_t 
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
-}
-// D[tmem] (+)= A[smem] B[smem]^T and D[tmem] (+)= A[tmem] B[smem]^T, 16-bit operands.
-__device__ __forceinline__ void mma_16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(
-          d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -141,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const rg_kv_cache& c = p.P.p.c;
   const rg_paged_attention_args& a = p.P.p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hk = blockIdx.y, b = blockIdx.z, group = (int)p.P.group.d;
   grid_launch_dependents();
 
@@ -196,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   // S_g (and P_g over its first 64 columns) at 128 g, O_g at 256 + D g
 
   // A softmax thread holds its row's 128 scores.  The launch gives 384 x 168 = 64512 registers;
@@ -227,70 +203,68 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tok0 = p.page_log2 >= 0 ? 0 : key0 - (int)p.P.page.div((uint32_t)key0) * c.page_size;
       for (int which = 0; which < 2; ++which, ++op) {
         const int st = op % C::kStages;
-        if (lane == 0) {
-          ok = mbar_wait_tight(&empty[st], ((op / C::kStages) & 1) ^ 1, abort, p.wait_ns);
-          if (ok) mbar_arrive_expect_tx(&full[st], (uint32_t)(pages * p.box * 128 * C::kHalves));
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = warp_wait(&empty[st], ((op / C::kStages) & 1) ^ 1, abort, p.wait_ns);
         if (!ok) break;
-        uint8_t* dst = ring + st * C::kOperand;
-        for (int i = lane; i < ((pages * C::kHalves + 31) & ~31); i += 32) {
-          const int j = i / C::kHalves, half = i % C::kHalves;
-          const int pg = __shfl_sync(0xffffffffu, page, j & 31);
-          if (j < pages)
-            tma_load_4d(dst + half * C::kSub + j * p.box * 128, which ? &map_v : &map_k, &full[st], half * 64, tok0, hk,
-                        pg);
+        expect_tx_elect(&full[st], (uint32_t)(pages * p.box * 128 * C::kHalves));
+        const uint32_t dst = smem_addr(ring) + st * C::kOperand;
+        for (int j = 0; j < pages; ++j) {
+          const int pg = __shfl_sync(0xffffffffu, page, j);
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half)
+            tma_load_4d_elect(dst + half * C::kSub + j * p.box * 128, which ? &map_v : &map_k, &full[st], half * 64,
+                              tok0, hk, pg);
         }
       }
     }
-    if (*abort && lane == 0) {  // a copy still on its way lands before the CTA leaves
+    if (*abort) {  // a copy still on its way lands before the CTA leaves
       volatile int never = 0;
       for (int s = 0; s < C::kStages && s < op; ++s) {
         const int o = op - 1 - s;
-        mbar_wait(&full[o % C::kStages], (o / C::kStages) & 1, &never, kDrainNs);
+        warp_wait(&full[o % C::kStages], (o / C::kStages) & 1, &never, kDrainNs);
       }
     }
   } else if (warp == 1) {
     // ---------------- products ----------------
-    if (lane == 0 && tiles > 0) {
+    if (tiles > 0) {
       constexpr uint32_t id_s = idesc_16<T>(kTile, kTile, false), id_o = idesc_16<T>(kTile, D, true);
       const uint32_t sq = smem_addr(smem), sr = smem_addr(ring);
       const auto wait_op = [&](int op) {
-        return mbar_wait_tight(&full[op % C::kStages], (op / C::kStages) & 1, abort, p.wait_ns);
+        return warp_wait(&full[op % C::kStages], (op / C::kStages) & 1, abort, p.wait_ns);
       };
       const auto scores = [&](int g, int op) {
-        const uint32_t q = sq + g * C::kOperand, k = sr + (op % C::kStages) * C::kOperand;
+        const uint64_t q = desc_kmajor_sw128(sq + g * C::kOperand);
+        const uint64_t k = desc_kmajor_sw128(sr + (op % C::kStages) * C::kOperand);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          mma_16_ss(tmem + g * kTile, desc_kmajor_sw128(q + (i >> 2) * C::kSub + (i & 3) * 32),
-                    desc_kmajor_sw128(k + (i >> 2) * C::kSub + (i & 3) * 32), id_s, i != 0);
+        for (int i = 0; i < D / 16; ++i) {  // 16 dimensions on: in the descriptors' 16-byte units
+          const int at = (i >> 2) * (C::kSub >> 4) + (i & 3) * 2;
+          mma_16_ss_elect(tmem + g * kTile, q + at, k + at, id_s, i != 0);
+        }
       };
-      bool ok = mbar_wait_tight(q_ready, 0, abort, p.wait_ns) && wait_op(0);
+      bool ok = warp_wait(q_ready, 0, abort, p.wait_ns) && wait_op(0);
       if (ok) {
         tc_fence_after();
         for (int g = 0; g < groups; ++g) {
           scores(g, 0);
-          mma_commit(&s_full[g]);
+          commit_elect(&s_full[g]);
         }
-        mma_commit(&empty[0]);
+        commit_elect(&empty[0]);
       }
       for (int n = 0; n < tiles && ok; ++n) {
         const int vop = 2 * n + 1, kop = 2 * n + 2;
         const bool more = n + 1 < tiles;
         ok = wait_op(vop);
         if (ok && !more && tail) {
-          mbar_arrive(v_here);
-          ok = mbar_wait_tight(v_fixed, 0, abort, p.wait_ns);
+          arrive_elect(v_here);
+          ok = warp_wait(v_fixed, 0, abort, p.wait_ns);
         }
-        const uint32_t v = sr + (vop % C::kStages) * C::kOperand;
+        const uint64_t v = desc_mnmajor_sw128(sr + (vop % C::kStages) * C::kOperand, C::kSub);
         for (int g = 0; g < groups && ok; ++g) {
-          ok = mbar_wait_tight(&p_ready[g], n & 1, abort, p.wait_ns);
+          ok = warp_wait(&p_ready[g], n & 1, abort, p.wait_ns);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < kTile / 16; ++i)
-            mma_16_ts(tmem + 256 + g * D, tmem + g * kTile + i * 8, desc_mnmajor_sw128(v + i * 2048, C::kSub), id_o,
-                      (n | i) != 0);
+          for (int i = 0; i < kTile / 16; ++i)  // 16 keys on: two 1024-byte atoms
+            mma_16_ts_elect(tmem + 256 + g * D, tmem + g * kTile + i * 8, v + i * 128, id_o, (n | i) != 0);
           if (more) {
             if (g == 0) {
               ok = wait_op(kop);
@@ -299,16 +273,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             scores(g, kop);
           }
-          mma_commit(&s_full[g]);
+          commit_elect(&s_full[g]);
         }
         if (ok) {
-          mma_commit(&empty[vop % C::kStages]);
-          if (more) mma_commit(&empty[kop % C::kStages]);
+          commit_elect(&empty[vop % C::kStages]);
+          if (more) commit_elect(&empty[kop % C::kStages]);
         }
       }
-      mma_commit(done);
+      commit_elect(done);
       volatile int never = 0;  // all products have completed before TMEM is freed
-      mbar_wait_tight(done, 0, &never, kDrainNs);
+      warp_wait(done, 0, &never, kDrainNs);
     }
   } else if (warp == 2) {
     // ---------------- V past the last key ----------------

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int num_tiles = p.tiles_m * p.tiles_n;
@@ -277,67 +277,66 @@ __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1)
   __syncthreads();
   cluster_sync();  // the peer's barriers exist before anything arrives on them
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      int issued = 0;
-      for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
-        int mb, nb;
-        pair_tile(tile, p, mb, nb);
-        for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait_tight(&empty[stage], phase ^ 1, abort, p.wait_ns)) { ok = false; break; }
-          if (!p.starve) {
-            uint8_t* sa = smem + stage * p.stage_bytes;
-            if (rank == 0)
-              mbar_arrive_expect_tx(&full[stage], (uint32_t)(p.a_ctas * p.a_rows * kBK + 2 * kBBytes));
-            const uint32_t bar = cluster_addr(&full[stage], 0);
-            tma_load_2d_pair(sa + p.a_rows * kBK, &map_w, bar, kb * kBK, nb * BN + (int)rank * (BN / 2));
-            if ((int)rank < p.a_ctas) {
-              if (issued == 0) grid_dependency_wait();  // W may be read before the quantizer is done, A not
-              tma_load_2d_pair(sa, &map_a, bar, kb * kBK, mb * 256 + (int)rank * 128);
-            }
-            ++issued;
+    const uint32_t ring = smem_addr(smem);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    int issued = 0;
+    for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
+      int mb, nb;
+      pair_tile(tile, p, mb, nb);
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        if (!warp_wait(&empty[stage], phase ^ 1, abort, p.wait_ns)) { ok = false; break; }
+        if (!p.starve) {
+          const uint32_t sa = ring + stage * p.stage_bytes;
+          if (rank == 0) expect_tx_elect(&full[stage], (uint32_t)(p.a_ctas * p.a_rows * kBK + 2 * kBBytes));
+          const uint32_t bar = cluster_addr(&full[stage], 0);
+          tma_load_2d_pair_elect(sa + p.a_rows * kBK, &map_w, bar, kb * kBK, nb * BN + (int)rank * (BN / 2));
+          if ((int)rank < p.a_ctas) {
+            if (issued == 0) grid_dependency_wait();  // W may be read before the quantizer is done, A not
+            tma_load_2d_pair_elect(sa, &map_a, bar, kb * kBK, mb * 256 + (int)rank * 128);
           }
-          if (++stage == p.stages) { stage = 0; phase ^= 1; }
+          ++issued;
         }
-      }
-      // Drain: the products that read the last stages arrive on `empty` here, so no copy or
-      // arrival is on its way to this CTA when it leaves.
-      volatile int never = 0;
-      for (int s = 0; s < p.stages && s < issued; ++s) {
-        stage = stage == 0 ? p.stages - 1 : stage - 1;
-        if (stage == p.stages - 1) phase ^= 1;
-        mbar_wait_tight(&empty[stage], phase, &never, kDrainNs);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
     }
+    // Drain: the products that read the last stages arrive on `empty` here, so no copy or
+    // arrival is on its way to this CTA when it leaves.
+    volatile int never = 0;
+    for (int s = 0; s < p.stages && s < issued; ++s) {
+      stage = stage == 0 ? p.stages - 1 : stage - 1;
+      if (stage == p.stages - 1) phase ^= 1;
+      warp_wait(&empty[stage], phase, &never, kDrainNs);
+    }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = idesc_i8(256, BN);
+      const uint32_t ring = smem_addr(smem);
       int stage = 0, iter = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += pairs, ++iter) {
         const int buf = iter & 1;
-        if (!mbar_wait_tight(&tempty[buf], ((iter >> 1) & 1) ^ 1, abort, p.wait_ns)) break;
+        if (!warp_wait(&tempty[buf], ((iter >> 1) & 1) ^ 1, abort, p.wait_ns)) break;
         tc_fence_after();
         for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait_tight(&full[stage], phase, abort, p.wait_ns)) { ok = false; break; }
+          if (!warp_wait(&full[stage], phase, abort, p.wait_ns)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_addr(smem + stage * p.stage_bytes), sb = sa + p.a_rows * kBK;
+          const uint32_t sa = ring + stage * p.stage_bytes;
+          const uint64_t da = desc_kmajor_sw128(sa), db = desc_kmajor_sw128(sa + p.a_rows * kBK);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 32; ++kk)
-            mma_i8_pair(tmem + (uint32_t)(buf * BN), desc_kmajor_sw128(sa + kk * 32),
-                        desc_kmajor_sw128(sb + kk * 32), idesc, (kb | kk) != 0);
-          mma_commit_pair(&empty[stage]);
+          for (int kk = 0; kk < kBK / 32; ++kk)  // 32 bytes on: 2 in the descriptors' 16-byte units
+            mma_i8_pair_elect(tmem + (uint32_t)(buf * BN), da + 2 * kk, db + 2 * kk, idesc, (kb | kk) != 0);
+          commit_pair_elect(&empty[stage]);
           if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
-        if (ok) mma_commit_pair(&tfull[buf]);
+        if (ok) commit_pair_elect(&tfull[buf]);
       }
-      mma_commit_pair(done);
+      commit_pair_elect(done);
     }
   } else {
     const int q = warp & 3;               // TMEM lane quadrant this warp may access
@@ -490,7 +489,7 @@ __global__ void __launch_bounds__(kFewThreads)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const TokenGemmArgs& g = p.g;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % p.splits;
   const int64_t n0 = (int64_t)(blockIdx.x / p.splits) * 128, t0 = (int64_t)blockIdx.y * p.tokens;
   const int tokens = (int)min((int64_t)p.tokens, g.m - t0);
@@ -511,54 +510,54 @@ __global__ void __launch_bounds__(kFewThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
-    if (lane == 0 && !p.starve) {
+    if (!p.starve) {
+      const uint32_t ring = smem_addr(smem);
       const uint32_t bytes = (uint32_t)(128 + p.box_rows) * kBK;
       const int first = min(p.stages, kb1 - kb0);
       for (int s = 0; s < first; ++s) {
-        mbar_arrive_expect_tx(&full[s], bytes);
-        tma_load_2d(smem + s * p.stage_bytes, &map_w, &full[s], (kb0 + s) * kBK, (int)n0);
+        expect_tx_elect(&full[s], bytes);
+        tma_load_2d_elect(ring + s * p.stage_bytes, &map_w, &full[s], (kb0 + s) * kBK, (int)n0);
       }
       grid_dependency_wait();
       for (int s = 0; s < first; ++s)
-        tma_load_2d(smem + s * p.stage_bytes + 128 * kBK, &map_a, &full[s], (kb0 + s) * kBK, (int)t0);
+        tma_load_2d_elect(ring + s * p.stage_bytes + 128 * kBK, &map_a, &full[s], (kb0 + s) * kBK, (int)t0);
       int stage = 0;
       uint32_t phase = 0;  // of the use before: its product empties the stage
       for (int kb = kb0 + first; kb < kb1; ++kb) {
-        if (!mbar_wait_tight(&empty[stage], phase, abort, p.wait_ns)) break;
-        uint8_t* sw = smem + stage * p.stage_bytes;
-        mbar_arrive_expect_tx(&full[stage], bytes);
-        tma_load_2d(sw, &map_w, &full[stage], kb * kBK, (int)n0);
-        tma_load_2d(sw + 128 * kBK, &map_a, &full[stage], kb * kBK, (int)t0);
+        if (!warp_wait(&empty[stage], phase, abort, p.wait_ns)) break;
+        const uint32_t sw = ring + stage * p.stage_bytes;
+        expect_tx_elect(&full[stage], bytes);
+        tma_load_2d_elect(sw, &map_w, &full[stage], kb * kBK, (int)n0);
+        tma_load_2d_elect(sw + 128 * kBK, &map_a, &full[stage], kb * kBK, (int)t0);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
       // Drain: a copy still on its way (after a wait gave up) lands before the CTA leaves.
       if (*abort) {
         volatile int never = 0;
-        for (int s = 0; s < first; ++s) mbar_wait(&full[s], s < stage ? phase ^ 1 : phase, &never, kDrainNs);
+        for (int s = 0; s < first; ++s) warp_wait(&full[s], s < stage ? phase ^ 1 : phase, &never, kDrainNs);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_i8(128, p.n_cols);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_tight(&full[stage], phase, abort, p.wait_ns)) break;
-        tc_fence_after();
-        const uint32_t sw = smem_addr(smem + stage * p.stage_bytes), sx = sw + 128 * kBK;
+    const uint32_t idesc = idesc_i8(128, p.n_cols), ring = smem_addr(smem);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(&full[stage], phase, abort, p.wait_ns)) break;
+      tc_fence_after();
+      const uint32_t sw = ring + stage * p.stage_bytes;
+      const uint64_t dw = desc_kmajor_sw128(sw), dx = desc_kmajor_sw128(sw + 128 * kBK);
 #pragma unroll
-        for (int kk = 0; kk < kBK / 32; ++kk)
-          mma_i8(tmem, desc_kmajor_sw128(sw + kk * 32), desc_kmajor_sw128(sx + kk * 32), idesc, (kb - kb0) | kk);
-        mma_commit(&empty[stage]);
-        if (++stage == p.stages) { stage = 0; phase ^= 1; }
-      }
-      mma_commit(tfull);
-      volatile int never = 0;  // all products have completed before TMEM is freed
-      mbar_wait_tight(tfull, 0, &never, p.wait_ns + kDrainNs);
+      for (int kk = 0; kk < kBK / 32; ++kk)  // 32 bytes on: 2 in the descriptors' 16-byte units
+        mma_i8_elect(tmem, dw + 2 * kk, dx + 2 * kk, idesc, (kb - kb0) | kk);
+      commit_elect(&empty[stage]);
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
+    commit_elect(tfull);
+    volatile int never = 0;  // all products have completed before TMEM is freed
+    warp_wait(tfull, 0, &never, p.wait_ns + kDrainNs);
   } else {
     const bool got = mbar_wait_tight(tfull, 0, abort, p.wait_ns);
     if (!__all_sync(0xffffffffu, got)) *abort = 1;
