@@ -1,10 +1,12 @@
-"""Builds librg_npu.so (all CUDA kernels + the C ABI) in-tree for sm_100a."""
+"""Builds librg_npu.so (all CUDA kernels + the C ABI) in-tree for sm_100a, and the binding of
+its serving entry points to torch tensors (_serving_bind.so)."""
 from __future__ import annotations
 
 import glob
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -12,6 +14,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librg_npu.so")
+BIND_SRC = os.path.join(HERE, "bind", "serving_bind.cpp")
+BIND = os.path.join(HERE, "_serving_bind.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -49,12 +53,40 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _torch_dir() -> str:
+    import importlib.util
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("torch not found")
+    return list(spec.submodule_search_locations)[0]
+
+
+def build_binding() -> str:
+    """Compiles bind/serving_bind.cpp against torch's headers and links it to librg_npu.so."""
+    header = os.path.join(ROOT, "include", "rg_npu.h")
+    if os.path.exists(BIND) and os.path.getmtime(BIND) >= max(os.path.getmtime(f) for f in (BIND_SRC, header)):
+        return BIND
+    torch = _torch_dir()
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
+           "-I", os.path.join(torch, "include"), "-I", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), BIND_SRC, "-o", BIND,
+           "-L", os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+           "-L", HERE, "-l:librg_npu.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(torch, "lib")]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {BIND} failed:\n{r.stdout}\n{r.stderr}")
+    return BIND
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cpp")))
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(_compile, srcs))
     if os.path.exists(LIB) and os.path.getmtime(LIB) >= max(os.path.getmtime(o) for o in objs):
+        build_binding()
         return LIB
     _, libdir = nccl_dirs()
     cmd = [NVCC] + ARCH + ["-shared", "-o", LIB] + objs + [
@@ -62,6 +94,7 @@ def build(verbose: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_binding()
     if verbose:
         print("built", LIB)
     return LIB
