@@ -27,6 +27,7 @@ whole batch with one scale, src/inference/npu.rs:312).
 from __future__ import annotations
 
 import ctypes as C
+from dataclasses import dataclass
 
 import torch
 
@@ -148,3 +149,113 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (shared in order); head_dim 64, 96, 128 or 256.  ``max_q_len`` and ``max_kv_len`` (default:
     what the table can hold) bound the lengths; ``scale`` defaults to 1 / sqrt(head_dim)."""
     return _bind.attention(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q_len, max_kv_len, scale, causal, out)
+
+
+@dataclass
+class Step:
+    """The index tensors of one batch of new tokens, in the order of the sequences given to
+    :meth:`PagedKvCache.extend`; every layer of a model uses the same ones."""
+    positions: torch.Tensor     # int32 [tokens]
+    slots: torch.Tensor         # int64 [tokens]
+    block_table: torch.Tensor   # int32 [batch, max_pages]
+    kv_len: torch.Tensor        # int32 [batch], the new tokens included
+    cu_q: torch.Tensor          # int32 [batch + 1]
+    max_q_len: int
+    max_kv_len: int
+
+
+class PagedKvCache:
+    """The pages of a model's layers and which sequence holds which.  ``k[layer]`` and
+    ``v[layer]`` are [pages, page_size, kv_heads, head_dim]; a page index means the same page in
+    every layer.  The bookkeeping is on the host; :meth:`extend` makes one step's index tensors
+    with one copy to the device."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if min(layers, pages, page_size, kv_heads, head_dim) <= 0:
+            raise ValueError("layers, pages, page_size, kv_heads and head_dim have to be positive")
+        self.page_size = page_size
+        self.k = [torch.zeros((pages, page_size, kv_heads, head_dim), dtype=dtype, device=device) for _ in range(layers)]
+        self.v = [torch.zeros_like(k) for k in self.k]
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages: dict[int, list[int]] = {}
+        self._len: dict[int, int] = {}
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, sequence: int) -> int:
+        """Tokens of ``sequence`` (0 when it is unknown)."""
+        return self._len.get(sequence, 0)
+
+    def release(self, sequence: int) -> None:
+        """Gives the sequence's pages back.  Work that reads them has to be ordered before work
+        that a later step gives them to (one stream does)."""
+        self._free.extend(reversed(self._pages.pop(sequence, [])))
+        self._len.pop(sequence, None)
+
+    def extend(self, new_tokens: dict[int, int]) -> Step:
+        """Room for ``new_tokens[sequence]`` more tokens of each sequence (made when unknown), and
+        the step's index tensors.  Nothing changes when the pages do not suffice (``MemoryError``)."""
+        page = self.page_size
+        if not new_tokens or any(n < 0 for n in new_tokens.values()):
+            raise ValueError("new_tokens: a count >= 0 for one sequence at least is needed")
+        need = {s: -(-(self.length(s) + n) // page) - len(self._pages.get(s, ())) for s, n in new_tokens.items()}
+        if sum(need.values()) > len(self._free):
+            raise MemoryError(f"{sum(need.values())} pages are needed, {len(self._free)} are free")
+        positions, slots, kv_len, cu_q = [], [], [], [0]
+        for s, n in new_tokens.items():
+            mine = self._pages.setdefault(s, [])
+            mine += [self._free.pop() for _ in range(need[s])]
+            first = self.length(s)
+            self._len[s] = first + n
+            positions += range(first, first + n)
+            slots += [mine[p // page] * page + p % page for p in range(first, first + n)]
+            kv_len.append(first + n)
+            cu_q.append(cu_q[-1] + n)
+        batch, tokens = len(kv_len), len(slots)
+        width = max(1, max(len(self._pages[s]) for s in new_tokens))
+        table = [x for s in new_tokens for x in self._pages[s] + [0] * (width - len(self._pages[s]))]
+        # one buffer, the 64-bit slots first
+        host = torch.empty(2 * tokens + tokens + 2 * batch + 1 + len(table), dtype=torch.int32,
+                           pin_memory=self.k[0].is_cuda)
+        host[:2 * tokens].view(torch.int64).copy_(torch.tensor(slots, dtype=torch.int64))
+        host[2 * tokens:].copy_(torch.tensor(positions + kv_len + cu_q + table, dtype=torch.int32))
+        dev = host.to(self.k[0].device, non_blocking=True)
+        slots_t, rest = dev[:2 * tokens].view(torch.int64), dev[2 * tokens:]
+        pos_t, kv_t, cu_t, table_t = rest.split([tokens, batch, batch + 1, len(table)])
+        return Step(pos_t, slots_t, table_t.view(batch, width), kv_t, cu_t,
+                    max(new_tokens.values()), max(kv_len))
+
+
+class DecoderAttention:
+    """Causal multi-head attention of a decoder with i8 projections: the reference's
+    MultiHeadAttention (src/nn/attention.rs:162-196) given rotary positions, a paged cache,
+    query heads that share key heads, and a quantization scale per token and channel.
+
+    ``wqkv`` [(heads + 2 kv_heads) head_dim, d] (query, key, value rows) and ``wo``
+    [d, heads head_dim] are float tensors on the device, quantized once here."""
+
+    def __init__(self, wqkv: torch.Tensor, wo: torch.Tensor, heads: int, kv_heads: int, table: torch.Tensor,
+                 bqkv: torch.Tensor | None = None, bo: torch.Tensor | None = None, interleaved: bool = False):
+        total = heads + 2 * kv_heads
+        if heads <= 0 or kv_heads <= 0 or heads % kv_heads or wqkv.shape[0] % total:
+            raise ValueError(f"wqkv {tuple(wqkv.shape)} does not split into {heads} + 2 x {kv_heads} heads")
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, wqkv.shape[0] // total
+        if wo.shape[1] != heads * self.head_dim:
+            raise ValueError(f"wo {tuple(wo.shape)} does not take {heads} heads of {self.head_dim}")
+        self.wqkv, self.sqkv = quantize_weight_i8(wqkv)
+        self.wo, self.so = quantize_weight_i8(wo)
+        self.bqkv, self.bo, self.table, self.interleaved = bqkv, bo, table, interleaved
+
+    def __call__(self, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, step: Step) -> torch.Tensor:
+        """x [tokens, d] of the step's new tokens -> [tokens, d]; their keys and values are appended."""
+        h, hk = self.heads, self.kv_heads
+        y = linear_i8_token(x, self.wqkv, self.sqkv, bias=self.bqkv, out_dtype=k_cache.dtype)
+        y = y.view(x.shape[0], h + 2 * hk, self.head_dim)
+        q = kv_append(y[:, h:h + hk], y[:, h + hk:], k_cache, v_cache, step.slots, positions=step.positions,
+                      table=self.table, interleaved=self.interleaved, q=y[:, :h])
+        o = attention_paged(q, k_cache, v_cache, step.block_table, step.kv_len, step.cu_q, step.max_q_len,
+                            step.max_kv_len)
+        return linear_i8_token(o.view(x.shape[0], h * self.head_dim), self.wo, self.so, bias=self.bo, out_dtype=x.dtype)

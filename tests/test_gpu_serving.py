@@ -658,3 +658,78 @@ def test_zero_sizes(gpu, sv):
     out = sv.attention_paged(e.half(), kc, kc, torch.empty((0, 1), dtype=torch.int32, device="cuda"), none, one,
                              max_q_len=1)
     assert out.shape == (0, 1, 64)
+
+
+# ---------------------------------------------------------------------------
+# the block, the cache's bookkeeping and the example
+# ---------------------------------------------------------------------------
+def test_decoder_attention_block(gpu, sv):
+    """The block against its parts: exact projections, the rotation, 64-bit attention."""
+    torch = gpu
+    d, h, hk, dim = 256, 6, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    table = sv.rope_table(512, dim)
+    block = sv.DecoderAttention(rand((h + 2 * hk) * dim, d) * 0.06, rand(d, h * dim) * 0.05, h, hk, table, bo=rand(d))
+    cache = sv.PagedKvCache(1, 40, 16, hk, dim)
+    x = {0: rand(150, d).bfloat16(), 1: rand(40, d).bfloat16()}
+    got = {s: [] for s in x}
+    for sizes in ({0: 100, 1: 3}, {0: 1, 1: 37}, {0: 49}):        # chunks and single tokens mixed
+        at = {s: cache.length(s) for s in sizes}
+        step = cache.extend(sizes)
+        out = block(torch.cat([x[s][at[s]:at[s] + n] for s, n in sizes.items()]), cache.k[0], cache.v[0], step)
+        for s, part in zip(sizes, out.split(list(sizes.values()))):
+            got[s].append(part)
+    sv.check()
+    for s, xs in x.items():
+        y = sv.linear_i8_token(xs, block.wqkv, block.sqkv).view(-1, h + 2 * hk, dim)
+        pos = np.arange(xs.shape[0])
+        turn = lambda t: torch.from_numpy(rotate_reference(t.float().cpu().numpy(), pos, table.cpu().numpy(),  # noqa: E731
+                                                           False)).bfloat16().cuda()
+        q, k, v = turn(y[:, :h]), turn(y[:, h:h + hk]), y[:, h + hk:]
+        o, _, _ = attention_reference(torch, q, k[None], v[None], torch.zeros((1, 1), dtype=torch.int32, device="cuda"),
+                                      [(len(pos), len(pos))], dim ** -0.5, True)
+        want = sv.linear_i8_token(o.bfloat16().view(len(pos), -1), block.wo, block.so, bias=block.bo).float()
+        off = (torch.cat(got[s]).float() - want).norm() / want.norm()
+        # attention within about 2^-8 of its reference, a step of 1 / 127 of its largest value where
+        # that changes a rounding, and the result's own 2^-9
+        assert off <= 0.01, float(off)
+
+
+def test_paged_cache_bookkeeping(gpu, sv):
+    torch = gpu
+    cache = sv.PagedKvCache(2, 5, 4, 1, 64, dtype=torch.float16)
+    step = cache.extend({7: 6, 9: 1})
+    assert step.positions.tolist() == [0, 1, 2, 3, 4, 5, 0] and step.cu_q.tolist() == [0, 6, 7]
+    assert step.kv_len.tolist() == [6, 1] and (step.max_q_len, step.max_kv_len) == (6, 6)
+    pages = [s // 4 for s in step.slots.tolist()]
+    assert pages[0] == pages[3] != pages[4] == pages[5] and len(set(pages)) == 3
+    assert step.block_table[0].tolist() == [pages[0], pages[4]] and step.block_table[1, 0] == pages[6]
+    with pytest.raises(MemoryError):
+        cache.extend({9: 20})
+    assert cache.length(9) == 1 and cache.free_pages == 2
+    step = cache.extend({9: 3, 7: 0})
+    assert [s // 4 for s in step.slots.tolist()] == [pages[6]] * 3 and step.positions.tolist() == [1, 2, 3]
+    cache.release(7)
+    assert cache.free_pages == 4 and cache.length(7) == 0
+    with pytest.raises(ValueError):
+        cache.extend({})
+
+
+def test_example_decodes_as_it_prefills(gpu, sv):
+    """The logits of decoded tokens are those of the same tokens prefilled as a prompt."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve_decoder.py")
+    spec = importlib.util.spec_from_file_location("serve_decoder", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    torch = gpu
+    model = m.Decoder(2, vocab=500, positions=512)
+    prompts = [[3, 1, 4, 1, 5], list(range(90)), [2] * 300]
+    tokens, logits = m.generate(model, prompts, 5, chunk=64)
+    longer = [p + t[:-1] for p, t in zip(prompts, tokens.tolist())]
+    _, again = m.generate(model, longer, 1, chunk=400)
+    # i8 steps that fall the other way after a 16-bit rounding: within a few percent
+    off = (logits[:, -1] - again[:, 0]).norm() / again[:, 0].norm()
+    assert off < 0.05, float(off)
