@@ -365,7 +365,7 @@ rg_status rg_gemm_i8_token(const int8_t* a, const float* a_scale, const int8_t* 
                            int64_t n, int64_t ld, const float* bias, int32_t act, float act_param, void* out,
                            int32_t out_dtype, int64_t ldo, int32_t* error_words, void* stream);
 /* The two in one call: x [m, k] (row stride ldx) against w [n, ld], ld >= k.  `workspace`
- * holds rg_linear_i8_token_workspace_size(m, ld) bytes, 256-byte aligned (NULL when that is
+ * holds rg_linear_i8_token_workspace_size(m, n, ld) bytes, 256-byte aligned (NULL when that is
  * 0), and is free again once the call's work on `stream` is done. */
 typedef struct rg_linear_token_args {
   const void* x; const int8_t* w; const float* w_scale; const float* bias; void* out;
@@ -373,7 +373,7 @@ typedef struct rg_linear_token_args {
   int32_t x_dtype, out_dtype, act;
   float act_param;
 } rg_linear_token_args;
-int64_t rg_linear_i8_token_workspace_size(int64_t m, int64_t ld);
+int64_t rg_linear_i8_token_workspace_size(int64_t m, int64_t n, int64_t ld);
 rg_status rg_linear_i8_token(const rg_linear_token_args* args, void* workspace, int32_t* error_words, void* stream);
 
 /* Rotary positions.  A table has one f32 row per position: rot_dim / 2 cosines, then

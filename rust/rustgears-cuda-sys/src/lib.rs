@@ -358,7 +358,7 @@ extern "C" {
     pub fn rg_gemm_i8_token(a: *const i8, a_scale: *const f32, w: *const i8, w_scale: *const f32, m: i64,
                             n: i64, ld: i64, bias: *const f32, act: i32, act_param: f32, out: *mut c_void,
                             out_dtype: i32, ldo: i64, error_words: *mut i32, stream: *mut c_void) -> rg_status;
-    pub fn rg_linear_i8_token_workspace_size(m: i64, ld: i64) -> i64;
+    pub fn rg_linear_i8_token_workspace_size(m: i64, n: i64, ld: i64) -> i64;
     pub fn rg_linear_i8_token(args: *const rg_linear_token_args, workspace: *mut c_void, error_words: *mut i32,
                               stream: *mut c_void) -> rg_status;
     pub fn rg_rope_table_f32(scaling: *const rg_rope_scaling, positions: i64, rot_dim: i32, table: *mut f32,

@@ -257,7 +257,7 @@ PyObject* linear(PyObject* const* o) {
   dev.also(given);
   at::Tensor out = given ? *given : empty(shape, type, dev.index);
   if (m > 0) {
-    const int64_t need = rg_linear_i8_token_workspace_size(m, ld);
+    const int64_t need = rg_linear_i8_token_workspace_size(m, n, ld);
     at::Tensor space;
     if (need > 0) space = empty({need}, at::kByte, dev.index);
     a.x = r.data_ptr();

@@ -399,9 +399,10 @@ rg_status go(const AttnParams& A, cudaStream_t st) {
   return RG_OK;
 }
 
-// Rows of a block: 16 (one fragment, all warps on the keys) or 64.
+// Rows of a block: 16 (one fragment, all warps on the keys), or 64 where rows come in numbers.
+// Beside chunks the sequences of this kernel are decoding ones, mostly of few rows.
 inline int few_rows(const AttnParams& A) {
-  return std::min<int64_t>((int64_t)A.p.a.max_q_len * A.group.d, A.max_rows) <= 16 ? 16 : 64;
+  return (int64_t)A.p.a.max_q_len * A.group.d <= 16 || A.max_rows < INT_MAX ? 16 : 64;
 }
 template <typename T, int D>
 rg_status go_rows(const AttnParams& A, cudaStream_t st) {
@@ -455,7 +456,7 @@ void launch_join(const JoinParams& J, int64_t rows, cudaStream_t st) {
 int split_keys(int64_t blocks, int64_t tiles, int slots, double tile_us, int min_tiles, double join_us) {
   int best = 1;
   double least = 1e30;
-  for (int s = 1; s <= 64 && (s == 1 || tiles >= (int64_t)s * min_tiles); ++s) {
+  for (int s = 1; s <= 64 && (s == 1 || (tiles + s - 1) / s >= min_tiles); ++s) {
     const double t = (double)((blocks * s + slots - 1) / slots) * (3.0 + tile_us * (double)((tiles + s - 1) / s)) +
                      (s > 1 ? 2.0 + s * join_us : 0.0);
     if (t < 0.97 * least) {
@@ -501,13 +502,19 @@ rg_status make_plan(const PagedAttnArgs& p, Plan& L) {
   L.few_shape = {few_rows(A), d <= 128 ? 64 : 32, 1};
   L.many_shape = {kTcRows, kTcKeys, 1};
   if (L.few) {
-    const int64_t tiles = (std::min<int64_t>(L.rows, A.max_rows) + L.few_shape.rows - 1) / L.few_shape.rows;
-    L.few_shape.splits = split_keys(seqs * tiles, (p.a.max_kv_len + L.few_shape.keys - 1) / L.few_shape.keys, 296,
+    // (beside chunks: taken as one block for every other sequence)
+    const int64_t blocks = L.many ? (seqs + 1) / 2 : seqs * ((L.rows + L.few_shape.rows - 1) / L.few_shape.rows);
+    L.few_shape.splits = split_keys(blocks, (p.a.max_kv_len + L.few_shape.keys - 1) / L.few_shape.keys, 296,
                                     d <= 64 ? 0.4 : 0.8, 2, row_us);
   }
-  if (L.many)
-    L.many_shape.splits = split_keys(seqs * ((L.rows + kTcRows - 1) / kTcRows),
-                                     (p.a.max_kv_len + kTcKeys - 1) / kTcKeys, 148, 2.3, 2, row_us);
+  if (L.many) {
+    // blocks with work: what the tokens fill, and half a block for every sequence's rest
+    const int64_t most = seqs * ((L.rows + kTcRows - 1) / kTcRows);
+    const int64_t blocks = std::min<int64_t>(
+        most, (p.a.tokens * A.group.d / kTcRows + (p.a.batch + 1) / 2 + 1) * (int64_t)p.c.kv_heads);
+    L.many_shape.splits = split_keys(blocks, (p.a.max_kv_len + kTcKeys - 1) / kTcKeys, 148, d <= 64 ? 1.6 : 1.9, 2,
+                                     row_us);
+  }
   const int most = std::max(L.few ? L.few_shape.splits : 1, L.many ? L.many_shape.splits : 1);
   L.part_rows = most > 1 ? most * p.a.tokens * p.a.heads : 0;
   return RG_OK;

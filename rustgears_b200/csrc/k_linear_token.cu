@@ -161,6 +161,13 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // exponent and reciprocal (relative error below 2^-19, far under the result's own rounding):
 // 7 instructions a value instead of about 90, which would outlast the products of a
 // 4096-long reduction.
+__device__ __forceinline__ float smooth16(int32_t act, float x) {  // GELU or SiLU
+  // GELU: 0.5 x (1 + tanh u) = x / (1 + e^(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+  const float c1 = act == ACT_GELU ? -2.0f * 0.7978846f * 1.44269504f : -1.44269504f;
+  const float c3 = act == ACT_GELU ? c1 * 0.044715f : 0.0f;
+  return x * rcp_approx(1.0f + mma16::ex2(x * fmaf(x * x, c3, c1)));
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void activate(float (&y)[N], int32_t act, float param) {
   if (act == ACT_NONE) return;
@@ -170,15 +177,8 @@ __device__ __forceinline__ void activate(float (&y)[N], int32_t act, float param
     return;
   }
   if (sizeof(T) == 2 && (act == ACT_GELU || act == ACT_SILU)) {
-    // GELU: 0.5 x (1 + tanh u) = x / (1 + e^(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
-    const float c1 = act == ACT_GELU ? -2.0f * 0.7978846f * 1.44269504f : -1.44269504f;
-    const float c3 = act == ACT_GELU ? c1 * 0.044715f : 0.0f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float x = y[j];
-      const float e = mma16::ex2(x * fmaf(x * x, c3, c1));
-      y[j] = x * rcp_approx(1.0f + e);
-    }
+    for (int j = 0; j < N; ++j) y[j] = smooth16(act, y[j]);
     return;
   }
   if (act == ACT_GELU) {
@@ -664,6 +664,173 @@ __global__ void __launch_bounds__(kFewThreads)
   }
 }
 
+// ---------------------------------------------------------------------------
+// Up to 8 tokens in one launch.  Bound: latency, and the stream of W for wide layers.  Every
+// block quantizes the tokens itself (m k values, from L2) while its first loads of W are under
+// way, then multiplies its 16 rows of W with mma.sync m16n8k32: W goes from memory to the
+// product's registers directly.  A thread's 16 bytes of a row feed two products whose K order is
+// permuted the same way on both sides (sums of integers: any order).  The block's 8 warps take
+// 64-byte steps of K in turn, and their sums meet in shared memory.
+//   The quantizer and the split-K product as two launches take 6.1 us for one token through
+// 1024 -> 2816 where this takes 3.8.
+// ---------------------------------------------------------------------------
+constexpr int kSkinnyTokens = 8, kSkinnyThreads = 256, kSkinnyWarps = 8;
+// Measured against the two launches: 3.8 / 6.1 us at 1 x 1024 x 2816, 7.7 / 9.7 at 1 x 4096 x 4096,
+// 9.3 / 10 at 2 x 4096 x 4096, 11.8 / 10.3 at 4 x 4096 x 4096 (every block quantizes), 21.7 / 17.1 at
+// 1 x 4096 x 14336 (more tiles than blocks at once).
+constexpr int64_t kSkinnyValues = 8192;  // m * ld
+constexpr int kSkinnyBlocks = 148 * 3;
+
+struct SkinnyParams {
+  TokenGemmArgs g;
+  const void* x;
+  int64_t ldx;
+  int32_t k, m, pitch, vec;
+};
+
+__device__ __forceinline__ void mma_i8_16832(int32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename TX, typename TO>
+__global__ void __launch_bounds__(kSkinnyThreads, 3) k_linear_skinny(const SkinnyParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int32_t part[kSkinnyWarps][16][kSkinnyTokens];
+  __shared__ float peak[kSkinnyWarps], scales[kSkinnyTokens];
+  const TokenGemmArgs& g = p.g;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, t4 = lane & 3;
+  const int ld = (int)g.ld;
+  const int steps = (ld + 63) / 64;  // of K; this warp takes steps warp, warp + 8, ...
+  constexpr int U = 4;               // steps in flight
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const auto load_w = [&](int64_t row, int s) {  // 16 bytes of a row at step s
+    const int at = s * 64 + t4 * 16;
+    return row < g.n && at < ld ? __ldg(reinterpret_cast<const uint4*>(g.w + row * ld + at)) : zero;
+  };
+  uint4 w0[U], w1[U];
+  const int tile = blockIdx.x;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    w0[u] = load_w((int64_t)tile * 16 + gr, warp + u * kSkinnyWarps);
+    w1[u] = load_w((int64_t)tile * 16 + gr + 8, warp + u * kSkinnyWarps);
+  }
+
+  // ---- quantize: 8 / (m rounded to a power of two) warps per token ----
+  {
+    int slots = 1;
+    while (slots < p.m) slots *= 2;
+    const int per = kSkinnyWarps / slots, token = warp / per, share = (warp % per) * 32 + lane, step = per * 32;
+    constexpr int E = 16 / (int)sizeof(TX);
+    const TX* x = static_cast<const TX*>(p.x) + token * p.ldx;
+    const int chunks = ld / E;  // ld: a multiple of 16
+    const auto read = [&](int c, float (&f)[E]) {
+      const int at = c * E;
+      if (p.vec && at + E <= p.k) {
+        Pack<TX, E>::load(x + at, f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[j] = at + j < p.k ? ElemOf<TX>::to(x[at + j]) : 0.0f;
+      }
+    };
+    float amax = 0.0f;
+    if (token < p.m)
+      for (int c = share; c < chunks; c += step) {
+        float f[E];
+        read(c, f);
+#pragma unroll
+        for (int j = 0; j < E; ++j) amax = fmaxf(amax, fabsf(f[j]));
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (lane == 0) peak[warp] = amax;
+    __syncthreads();
+    for (int i = 0; i < per; ++i) amax = fmaxf(amax, peak[token * per + i]);
+    const float sc = quant_scale(amax), inv = quant_inv(sc);
+    if (warp % per == 0 && lane == 0) scales[token] = sc;
+    uint8_t* q = smem + token * p.pitch;
+    for (int c = share; c < chunks; c += step) {
+      struct alignas(E) Out {
+        int8_t b[E];
+      } u;
+      float f[E];
+      if (token < p.m) {
+        read(c, f);
+#pragma unroll
+        for (int j = 0; j < E; ++j) u.b[j] = (int8_t)quant1_bounded(f[j], inv);
+        *reinterpret_cast<Out*>(q + c * E) = u;
+      }
+    }
+  }
+  __syncthreads();
+
+  const uint8_t* xq = smem + min(gr, p.m - 1) * p.pitch + t4 * 16;
+  const bool has = gr < p.m;
+  {
+    const int64_t row0 = (int64_t)tile * 16 + gr;
+    int32_t d[4] = {0, 0, 0, 0};
+    for (int s = warp; s < steps; s += U * kSkinnyWarps) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int now = s + u * kSkinnyWarps;
+        const uint4 a = w0[u], b = w1[u];
+        const int then = now + U * kSkinnyWarps;  // the step that takes these registers next
+        if (then < steps) {
+          w0[u] = load_w(row0, then);
+          w1[u] = load_w(row0 + 8, then);
+        }
+        if (now * 64 < ld) {
+          const uint4 v = has && now * 64 + t4 * 16 < ld ? *reinterpret_cast<const uint4*>(xq + now * 64) : zero;
+          mma_i8_16832(d, a.x, b.x, a.y, b.y, v.x, v.y);
+          mma_i8_16832(d, a.z, b.z, a.w, b.w, v.z, v.w);
+        }
+      }
+    }
+    // d: rows gr and gr + 8, tokens 2 t4 and 2 t4 + 1
+    *reinterpret_cast<int2*>(&part[warp][gr][2 * t4]) = make_int2(d[0], d[1]);
+    *reinterpret_cast<int2*>(&part[warp][gr + 8][2 * t4]) = make_int2(d[2], d[3]);
+    __syncthreads();
+    if (tid < 128) {
+      const int r = tid & 15, t = tid >> 4;
+      const int64_t n = (int64_t)tile * 16 + r;
+      if (t < p.m && n < g.n) {
+        int32_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < kSkinnyWarps; ++i) sum += part[i][r][t];
+        const float y = dequant(sum, __fmul_rn(scales[t], __ldg(g.w_scale + n)), g.bias ? __ldg(g.bias + n) : 0.0f);
+        static_cast<TO*>(g.out)[t * g.ldo + n] =
+            ElemOf<TO>::from(sizeof(TO) == 2 && (g.act == ACT_GELU || g.act == ACT_SILU)
+                                 ? smooth16(g.act, y)
+                                 : act_apply(g.act, g.act_param, y));
+      }
+    }
+  }
+}
+
+template <typename TX, typename TO>
+rg_status go_skinny(const TokenGemmArgs& a, const void* x, int64_t k, int64_t ldx, cudaStream_t st) {
+  SkinnyParams p;
+  p.g = a;
+  p.x = x;
+  p.ldx = ldx;
+  p.k = (int32_t)k;
+  p.m = (int32_t)a.m;
+  p.pitch = (int32_t)a.ld + 16;
+  p.vec = (((uintptr_t)x | (uintptr_t)(ldx * (int64_t)sizeof(TX))) & 15) == 0;
+  k_linear_skinny<TX, TO><<<(unsigned)((a.n + 15) / 16), kSkinnyThreads, p.m * p.pitch, st>>>(p);
+  return RG_OK;
+}
+
+template <typename TX>
+rg_status go_skinny_out(const TokenGemmArgs& a, const void* x, int64_t k, int64_t ldx, cudaStream_t st) {
+  if (a.out_dtype == RG_DTYPE_F32) return go_skinny<TX, float>(a, x, k, ldx, st);
+  return a.out_dtype == RG_DTYPE_F16 ? go_skinny<TX, __half>(a, x, k, ldx, st)
+                                     : go_skinny<TX, __nv_bfloat16>(a, x, k, ldx, st);
+}
+
 bool operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t ld, int box_rows) {
   const auto fn = tma_encode_fn();
   if (!fn) return false;
@@ -794,6 +961,17 @@ void launch_quantize_token(const void* x, int32_t dtype, int64_t rows, int64_t k
   if (dtype == RG_DTYPE_F32) quantize<float>(x, rows, k, ldx, q, ldq, scale, st);
   else if (dtype == RG_DTYPE_F16) quantize<__half>(x, rows, k, ldx, q, ldq, scale, st);
   else quantize<__nv_bfloat16>(x, rows, k, ldx, q, ldq, scale, st);
+}
+
+bool linear_skinny_takes(int64_t m, int64_t n, int64_t ld) {
+  return m <= kSkinnyTokens && m * ld <= kSkinnyValues && n <= 16 * kSkinnyBlocks;
+}
+
+rg_status launch_linear_skinny(const TokenGemmArgs& a, const void* x, int32_t dtype, int64_t k, int64_t ldx,
+                               cudaStream_t st) {
+  if (dtype == RG_DTYPE_F32) return go_skinny_out<float>(a, x, k, ldx, st);
+  return dtype == RG_DTYPE_F16 ? go_skinny_out<__half>(a, x, k, ldx, st)
+                               : go_skinny_out<__nv_bfloat16>(a, x, k, ldx, st);
 }
 
 rg_status launch_gemm_token(const TokenGemmArgs& a, cudaStream_t st) {

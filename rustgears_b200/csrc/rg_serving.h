@@ -99,6 +99,10 @@ struct TokenGemmArgs {
   int32_t starve = 0;    // test hook: issue no operand loads, so the waits run out
 };
 rg_status launch_gemm_token(const TokenGemmArgs& a, cudaStream_t st);
+// Quantizer and product in one launch for a few tokens (a, a_scale unused).
+bool linear_skinny_takes(int64_t m, int64_t n, int64_t ld);
+rg_status launch_linear_skinny(const TokenGemmArgs& a, const void* x, int32_t dtype, int64_t k, int64_t ldx,
+                               cudaStream_t st);
 
 // ---- rotary positions and the paged append (k_rope.cu) --------------------------
 // Three groups of heads per token: q heads (rotated, stored by strides), then kv_heads

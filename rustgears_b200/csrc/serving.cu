@@ -38,17 +38,14 @@ bool is_dtype(int32_t dt) { return dt == RG_DTYPE_F32 || dt == RG_DTYPE_F16 || d
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-rg_status check_quantize(const char* f, const void* x, int32_t dt, int64_t rows, int64_t k, int64_t ldx,
-                         const int8_t* q, int64_t ldq, const float* scale) {
+rg_status check_rows(const char* f, const void* x, int32_t dt, int64_t rows, int64_t k, int64_t ldx, int64_t ldq) {
   if (!is_dtype(dt)) return refuse(RG_ERR_INVALID_ARG, "%s: unknown x dtype %d", f, dt);
   if (rows < 0 || rows > INT_MAX || k <= 0 || ldx < k || ldq < k || (ldq & 15))
     return refuse(RG_ERR_INVALID_ARG,
                   "%s: rows %lld, k %lld, ldx %lld, ld %lld (ldx >= k, ld >= k and a multiple of 16 wanted)", f,
                   (long long)rows, (long long)k, (long long)ldx, (long long)ldq);
-  if (rows == 0) return RG_OK;
-  if (!x || !q || !scale) return refuse(RG_ERR_INVALID_ARG, "%s: null argument", f);
-  if (!aligned(x, dtype_size(dt)) || !aligned(q, 16) || !aligned(scale, 4))
-    return refuse(RG_ERR_INVALID_ARG, "%s: x must be aligned to its type, the i8 rows to 16 bytes", f);
+  if (rows > 0 && !x) return refuse(RG_ERR_INVALID_ARG, "%s: null argument", f);
+  if (rows > 0 && !aligned(x, dtype_size(dt))) return refuse(RG_ERR_INVALID_ARG, "%s: x must be aligned to its type", f);
   return RG_OK;
 }
 
@@ -105,10 +102,14 @@ extern "C" {
 
 rg_status rg_quantize_token_i8(const void* x, int32_t x_dtype, int64_t rows, int64_t k, int64_t ldx, int8_t* q,
                                int64_t ldq, float* scale, void* stream) {
-  RG_CHECK(check_quantize("rg_quantize_token_i8", x, x_dtype, rows, k, ldx, q, ldq, scale));
+  const char* f = "rg_quantize_token_i8";
+  RG_CHECK(check_rows(f, x, x_dtype, rows, k, ldx, ldq));
   if (rows == 0) return RG_OK;
+  if (!q || !scale) return refuse(RG_ERR_INVALID_ARG, "%s: null argument", f);
+  if (!aligned(q, 16) || !aligned(scale, 4))
+    return refuse(RG_ERR_INVALID_ARG, "%s: the i8 rows must be aligned to 16 bytes", f);
   launch_quantize_token(x, x_dtype, rows, k, ldx, q, ldq, scale, (cudaStream_t)stream);
-  return launched("rg_quantize_token_i8", RG_OK);
+  return launched(f, RG_OK);
 }
 
 rg_status rg_gemm_i8_token(const int8_t* a, const float* a_scale, const int8_t* w, const float* w_scale, int64_t m,
@@ -127,8 +128,8 @@ rg_status rg_gemm_i8_token(const int8_t* a, const float* a_scale, const int8_t* 
   return launched(f, launch_gemm_token(g, (cudaStream_t)stream));
 }
 
-int64_t rg_linear_i8_token_workspace_size(int64_t m, int64_t ld) {
-  if (m <= 0 || ld <= 0) return 0;
+int64_t rg_linear_i8_token_workspace_size(int64_t m, int64_t n, int64_t ld) {
+  if (m <= 0 || n <= 0 || ld <= 0 || linear_skinny_takes(m, n, ld)) return 0;
   return round_up(m * ld, 256) + round_up(m * (int64_t)sizeof(float), 256);
 }
 
@@ -137,18 +138,20 @@ rg_status rg_linear_i8_token(const rg_linear_token_args* p, void* workspace, int
   if (!p) return refuse(RG_ERR_INVALID_ARG, "%s: null arguments", f);
   RG_CHECK(check_gemm(f, p->w, p->w_scale, p->m, p->n, p->ld, p->bias, p->act, p->out, p->out_dtype, p->ldo,
                       error_words));
-  if (p->m > 0 && (!workspace || !aligned(workspace, 256)))
+  const bool skinny = linear_skinny_takes(p->m, p->n, p->ld);
+  if (p->m > 0 && !skinny && (!workspace || !aligned(workspace, 256)))
     return refuse(RG_ERR_INVALID_ARG, "%s: the workspace must be given and 256-byte aligned", f);
   int8_t* q = static_cast<int8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(p->m * p->ld, 256));
-  RG_CHECK(check_quantize(f, p->x, p->x_dtype, p->m, p->k, p->ldx, q, p->ld, scale));
+  RG_CHECK(check_rows(f, p->x, p->x_dtype, p->m, p->k, p->ldx, p->ld));
   if (p->m == 0) return RG_OK;
-  launch_quantize_token(p->x, p->x_dtype, p->m, p->k, p->ldx, q, p->ld, scale, (cudaStream_t)stream);
   TokenGemmArgs g;
   g.a = q; g.a_scale = scale; g.w = p->w; g.w_scale = p->w_scale; g.bias = p->bias;
   g.m = p->m; g.n = p->n; g.ld = p->ld; g.ldo = p->ldo; g.act = p->act; g.act_param = p->act_param;
   g.out = p->out; g.out_dtype = p->out_dtype; g.err = error_words; g.after_quantizer = 1;
   tc_wait_hook(&g.wait_ns, &g.starve);
+  if (skinny) return launched(f, launch_linear_skinny(g, p->x, p->x_dtype, p->k, p->ldx, (cudaStream_t)stream));
+  launch_quantize_token(p->x, p->x_dtype, p->m, p->k, p->ldx, q, p->ld, scale, (cudaStream_t)stream);
   return launched(f, launch_gemm_token(g, (cudaStream_t)stream));
 }
 

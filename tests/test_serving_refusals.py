@@ -66,8 +66,8 @@ def test_linear_needs_its_workspace():
 
 def test_linear_workspace_holds_rows_and_scales():
     L = _native.lib()
-    assert L.rg_linear_i8_token_workspace_size(0, 32) == 0
-    assert L.rg_linear_i8_token_workspace_size(300, 32) >= 300 * 32 + 300 * 4
+    assert L.rg_linear_i8_token_workspace_size(0, 8, 32) == 0
+    assert L.rg_linear_i8_token_workspace_size(300, 8, 32) >= 300 * 32 + 300 * 4
 
 
 @pytest.mark.parametrize("change,match", [
