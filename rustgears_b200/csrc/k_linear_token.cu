@@ -35,69 +35,121 @@ __device__ __forceinline__ void grid_launch_dependents() {
 // per row; the row stays in registers, as it was read, between its absmax and its rounding
 // (32 values a thread, 8192 a row); longer rows are read again, from L1 or L2.
 // ---------------------------------------------------------------------------
+// The low bytes of four integers.
+__device__ __forceinline__ uint32_t pack_i8(int32_t a, int32_t b, int32_t c, int32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+template <typename T>
+__device__ __forceinline__ T from_bits(uint16_t v);
+template <>
+__device__ __forceinline__ __half from_bits<__half>(uint16_t v) { return __ushort_as_half(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_bits<__nv_bfloat16>(uint16_t v) { return __ushort_as_bfloat16(v); }
+// Largest magnitude, NaN ignored; 16-bit values two at a time (their maximum is exact).
+template <typename T>
+struct AbsMax;
+template <>
+struct AbsMax<float> {
+  float m = 0.0f;
+  __device__ __forceinline__ void fold(float a, float b) { m = fmaxf(m, fmaxf(fabsf(a), fabsf(b))); }
+  __device__ __forceinline__ float value() const { return m; }
+};
+template <>
+struct AbsMax<__half> {
+  __half2 m = __half2half2(__ushort_as_half(0));
+  __device__ __forceinline__ void fold(__half a, __half b) { m = __hmax2(m, __habs2(__halves2half2(a, b))); }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <>
+struct AbsMax<__nv_bfloat16> {
+  __nv_bfloat162 m = __bfloat162bfloat162(__ushort_as_bfloat16(0));
+  __device__ __forceinline__ void fold(__nv_bfloat16 a, __nv_bfloat16 b) {
+    m = __hmax2(m, __habs2(__halves2bfloat162(a, b)));
+  }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads)
-    k_quantize_token(const T* __restrict__ x, int64_t k, int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
-                     float* __restrict__ scale) {
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 6 : 4)
+    k_quantize_token(const T* __restrict__ x, int64_t k, int64_t ldx, int8_t* __restrict__ q,
+                     int64_t ldq, float* __restrict__ scale) {
   constexpr int E = VEC ? 16 / (int)sizeof(T) : 4;  // values a thread handles at once
   constexpr int NREG = 32 / E;
-  struct alignas(16) Raw {
-    T e[E];
+  // A chunk as it was read: 32-bit words, taken apart where they are used (16-bit values would be
+  // unpacked behind each load, which then waits for it).
+  constexpr int W = E * (int)sizeof(T) / 4;
+  struct Raw {
+    uint32_t w[W];
+    __device__ __forceinline__ T at(int j) const {
+      if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+      else return from_bits<T>((uint16_t)(w[j / 2] >> (j % 2 * 16)));
+    }
   };
   __shared__ float red[kQuantThreads / 32];
   grid_launch_dependents();
-  const int64_t r = blockIdx.x;
-  x += r * ldx;
-  q += r * ldq;
   const int chunks = (int)(ldq / E);
-  const auto read = [&](int c) {
+  const auto read = [&](int64_t r, int c) {
     Raw v;
     const int64_t at = (int64_t)c * E;
+    const T* src = x + r * ldx;
     if (VEC && at + E <= k) {
-      v = *reinterpret_cast<const Raw*>(x + at);
-    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + at);
+      v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) v.e[j] = at + j < k ? x[at + j] : ElemOf<T>::from(0.0f);
+      for (int j = 0; j < E; ++j) v.w[j] = at + j < k ? __float_as_uint(src[at + j]) : 0u;
+    } else {
+      const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+      for (int j = 0; j < E; j += 2)
+        v.w[j / 2] = (at + j < k ? bits[at + j] : 0u) | (at + j + 1 < k ? (uint32_t)bits[at + j + 1] << 16 : 0u);
     }
     return v;
   };
+  const int64_t r = blockIdx.x;
   Raw keep[NREG];
 #pragma unroll
   for (int i = 0; i < NREG; ++i) {
     const int c = threadIdx.x + i * kQuantThreads;
-    if (c < chunks) keep[i] = read(c);
+    if (c < chunks) keep[i] = read(r, c);
   }
-  float amax = 0.0f;
-  const auto fold = [&](const Raw& v) {
+  {
+    AbsMax<T> peak;
+    const auto fold = [&](const Raw& v) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) amax = fmaxf(amax, fabsf(ElemOf<T>::to(v.e[j])));
-  };
+      for (int j = 0; j < E; j += 2) peak.fold(v.at(j), v.at(j + 1));
+    };
 #pragma unroll
-  for (int i = 0; i < NREG; ++i)
-    if (threadIdx.x + i * kQuantThreads < chunks) fold(keep[i]);
-  for (int c = threadIdx.x + NREG * kQuantThreads; c < chunks; c += kQuantThreads) fold(read(c));
+    for (int i = 0; i < NREG; ++i)
+      if (threadIdx.x + i * kQuantThreads < chunks) fold(keep[i]);
+    for (int c = threadIdx.x + NREG * kQuantThreads; c < chunks; c += kQuantThreads) fold(read(r, c));
+    float amax = peak.value();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-  __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kQuantThreads / 32; ++i) amax = fmaxf(amax, red[i]);
-  const float sc = quant_scale(amax), inv = quant_inv(sc);
-  if (threadIdx.x == 0) scale[r] = sc;
-  const auto write = [&](int c, const Raw& v) {
-    struct alignas(E) Out {
-      int8_t b[E];
-    } u;
+    for (int i = 0; i < kQuantThreads / 32; ++i) amax = fmaxf(amax, red[i]);
+    const float sc = quant_scale(amax), inv = quant_inv(sc);
+    if (threadIdx.x == 0) scale[r] = sc;
+    const auto write = [&](int c, const Raw& v) {
+      struct alignas(E) Out {
+        uint32_t w[E / 4];
+      } u;
 #pragma unroll
-    for (int j = 0; j < E; ++j) u.b[j] = (int8_t)quant1_bounded(ElemOf<T>::to(v.e[j]), inv);
-    *reinterpret_cast<Out*>(q + (int64_t)c * E) = u;
-  };
+      for (int j = 0; j < E; j += 4)
+        u.w[j / 4] = pack_i8(quant1_bounded(ElemOf<T>::to(v.at(j)), inv), quant1_bounded(ElemOf<T>::to(v.at(j + 1)), inv),
+                             quant1_bounded(ElemOf<T>::to(v.at(j + 2)), inv),
+                             quant1_bounded(ElemOf<T>::to(v.at(j + 3)), inv));
+      *reinterpret_cast<Out*>(q + r * ldq + (int64_t)c * E) = u;
+    };
 #pragma unroll
-  for (int i = 0; i < NREG; ++i) {
-    const int c = threadIdx.x + i * kQuantThreads;
-    if (c < chunks) write(c, keep[i]);
+    for (int i = 0; i < NREG; ++i) {
+      const int c = threadIdx.x + i * kQuantThreads;
+      if (c < chunks) write(c, keep[i]);
+    }
+    for (int c = threadIdx.x + NREG * kQuantThreads; c < chunks; c += kQuantThreads) write(c, read(r, c));
   }
-  for (int c = threadIdx.x + NREG * kQuantThreads; c < chunks; c += kQuantThreads) write(c, read(c));
 }
 
 template <typename T>
