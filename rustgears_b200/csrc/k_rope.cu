@@ -23,16 +23,18 @@ namespace {
 constexpr int kThreads = 256;
 
 template <typename TI, typename TO, int P, bool INTER>
-__global__ void __launch_bounds__(kThreads) k_rope(const RopeArgs a, int32_t tokens_per_block, int32_t units) {
-  // units: work items of one head (rot / 2P rotations, then (head_dim - rot) / 2P copies)
-  const int per_token = (a.heads + 2 * a.kv_heads) * units;
+__global__ void __launch_bounds__(kThreads)
+    k_rope(const RopeArgs a, int32_t tokens_per_block, FastDiv per_token, FastDiv units, FastDiv page_size) {
+  // units: work items of one head (rot / 2P rotations, then (head_dim - rot) / 2P copies);
+  // per_token: those of all heads
   const int i = blockIdx.y * kThreads + threadIdx.x;
-  if (i >= tokens_per_block * per_token) return;
-  const int64_t t = (int64_t)blockIdx.x * tokens_per_block + i / per_token;
+  const int within = (int)per_token.div((uint32_t)i);
+  if (within >= tokens_per_block) return;
+  const int64_t t = (int64_t)blockIdx.x * tokens_per_block + within;
   if (t >= a.tokens) return;
-  const int rem = i % per_token;
-  int h = rem / units;
-  const int u = rem % units;
+  const int rem = i - within * (int)per_token.d;
+  int h = (int)units.div((uint32_t)rem);
+  const int u = rem - h * (int)units.d;
 
   const TI* src;
   TO* dst;
@@ -56,7 +58,8 @@ __global__ void __launch_bounds__(kThreads) k_rope(const RopeArgs a, int32_t tok
       a.err[1] = 1;
       return;
     }
-    const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
+    const int64_t page = slot <= INT_MAX ? (int64_t)page_size.div((uint32_t)slot) : slot / a.page_size;
+    const int64_t off = slot - page * a.page_size;
     const bool value = h >= a.kv_heads;
     if (value) h -= a.kv_heads;
     src = value ? static_cast<const TI*>(a.v) + t * a.v_ts + h * a.v_hs
@@ -136,8 +139,9 @@ rg_status go(const RopeArgs& a, cudaStream_t st) {
   const int64_t blocks = (a.tokens + tpb - 1) / tpb;
   if (blocks > INT_MAX) return RG_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)blocks, (unsigned)((tpb * per_token + kThreads - 1) / kThreads));
-  if (a.interleaved) k_rope<TI, TO, P, true><<<grid, kThreads, 0, st>>>(a, tpb, units);
-  else k_rope<TI, TO, P, false><<<grid, kThreads, 0, st>>>(a, tpb, units);
+  const FastDiv by_token((uint32_t)per_token), by_head((uint32_t)units), by_page((uint32_t)a.page_size);
+  if (a.interleaved) k_rope<TI, TO, P, true><<<grid, kThreads, 0, st>>>(a, tpb, by_token, by_head, by_page);
+  else k_rope<TI, TO, P, false><<<grid, kThreads, 0, st>>>(a, tpb, by_token, by_head, by_page);
   return RG_OK;
 }
 

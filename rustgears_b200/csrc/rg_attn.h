@@ -5,21 +5,6 @@
 
 namespace rg {
 
-// n / d for 0 <= n < 2^31 by multiplication (Granlund and Montgomery, PLDI 1994):
-// m = floor(2^32 (2^l - d) / d) + 1, l = ceil(log2 d).
-struct FastDiv {
-  uint32_t d, m, s;
-  explicit FastDiv(uint32_t v = 1) : d(v) {
-    uint32_t l = 0;
-    while ((1ull << l) < v) ++l;
-    m = (uint32_t)(((1ull << 32) * ((1ull << l) - v)) / v + 1);
-    s = l;
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
-    return (uint32_t)(((uint64_t)__umulhi(n, m) + n) >> s);
-  }
-};
-
 struct AttnParams {
   PagedAttnArgs p;
   FastDiv page, group;
