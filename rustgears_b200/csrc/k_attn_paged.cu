@@ -449,16 +449,28 @@ void launch_join(const JoinParams& J, int64_t rows, cudaStream_t st) {
   else launch_join<T, 1>(J, rows, st);
 }
 
-// Splits of a launch of `blocks` blocks over `tiles` key tiles each, `slots` blocks running at
-// once: the least of rounds x (a block's start + its tiles) + the join, in microseconds; the
-// times were measured (a start of about 3, a join of about 2 and of 8 bytes a partial value at
-// 5 TB/s).
-int split_keys(int64_t blocks, int64_t tiles, int slots, double tile_us, int min_tiles, double join_us) {
+// How a launch's time depends on its splits, in microseconds (measured): a block's start, a key
+// tile, `slots` blocks at once.
+struct Pace {
+  int slots;
+  double start, tile;
+};
+
+// Splits of `blocks` blocks of at most `tiles` key tiles.  Blocks that all run at once take as
+// long as the longest; more of them take their sum over the slots, and half a longest block
+// until the last one ends: the host knows the longest sequence only, so the others of a batch
+// count as 0.6 of it.  The join costs about 2 us, and join_us a split for the partial rows.
+int split_keys(int64_t blocks, int64_t tiles, bool one_sequence, const Pace& pace, int min_tiles, double join_us) {
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= 64 && (s == 1 || (tiles + s - 1) / s >= min_tiles); ++s) {
-    const double t = (double)((blocks * s + slots - 1) / slots) * (3.0 + tile_us * (double)((tiles + s - 1) / s)) +
-                     (s > 1 ? 2.0 + s * join_us : 0.0);
+    const int64_t per = (tiles + s - 1) / s, n = blocks * s;
+    const double one = pace.start + pace.tile * (double)per;
+    double t = one;
+    if (n > pace.slots)
+      t = one_sequence ? (double)((n + pace.slots - 1) / pace.slots) * one
+                       : (double)n / pace.slots * (pace.start + 0.6 * pace.tile * (double)per) + 0.5 * one;
+    if (s > 1) t += 2.0 + s * join_us;
     if (t < 0.97 * least) {
       least = t;
       best = s;
@@ -504,16 +516,17 @@ rg_status make_plan(const PagedAttnArgs& p, Plan& L) {
   if (L.few) {
     // (beside chunks: taken as one block for every other sequence)
     const int64_t blocks = L.many ? (seqs + 1) / 2 : seqs * ((L.rows + L.few_shape.rows - 1) / L.few_shape.rows);
-    L.few_shape.splits = split_keys(blocks, (p.a.max_kv_len + L.few_shape.keys - 1) / L.few_shape.keys, 296,
-                                    d <= 64 ? 0.4 : 0.8, 2, row_us);
+    const Pace pace = {296, 2.5, d <= 64 ? 0.6 : d <= 96 ? 0.8 : 1.1};
+    L.few_shape.splits = split_keys(blocks, (p.a.max_kv_len + L.few_shape.keys - 1) / L.few_shape.keys,
+                                    p.a.batch == 1, pace, 2, row_us);
   }
   if (L.many) {
     // blocks with work: what the tokens fill, and half a block for every sequence's rest
     const int64_t most = seqs * ((L.rows + kTcRows - 1) / kTcRows);
     const int64_t blocks = std::min<int64_t>(
         most, (p.a.tokens * A.group.d / kTcRows + (p.a.batch + 1) / 2 + 1) * (int64_t)p.c.kv_heads);
-    L.many_shape.splits = split_keys(blocks, (p.a.max_kv_len + kTcKeys - 1) / kTcKeys, 148, d <= 64 ? 1.6 : 1.9, 2,
-                                     row_us);
+    const Pace pace = {148, 4.0, d <= 64 ? 1.6 : 1.9};
+    L.many_shape.splits = split_keys(blocks, (p.a.max_kv_len + kTcKeys - 1) / kTcKeys, p.a.batch == 1, pace, 2, row_us);
   }
   const int most = std::max(L.few ? L.few_shape.splits : 1, L.many ? L.many_shape.splits : 1);
   L.part_rows = most > 1 ? most * p.a.tokens * p.a.heads : 0;
