@@ -7,14 +7,20 @@
 //   P_g = 2^(S_g scale2 - m), rounded to the cache's type, written over S_g in TMEM
 //   O_g += P_g V    tcgen05, P from TMEM, V from shared memory as it was loaded (keys are the
 //                   product's K dimension: V is the "transposed" operand), O in TMEM
-// One thread per row does the softmax, so a row's maximum and sum need no exchange.  While one
+// One thread per row does the softmax, so a row's maximum and sum need no exchange; its 128
+// scores take 224 registers, which the control warps give up.  (Two threads per row on half the
+// keys each, 16 warps: 498 against 474 us at D = 128, 454 against 478 at D = 64.)  While one
 // group's exponentials run, the tensor cores work on the other group.  A new maximum rescales
 // O only when it exceeds the one in use by 2^8 (the sums stay exact: numerator and denominator
 // use the same m; 2^8 fits every type here), so O is almost never read back.
 //
 // Bound: per 128 x 128 tile and group 2 x 128 x 128 x D products (1024 clocks of the tensor
 // pipe at D = 128) against 16384 exponentials (1024 clocks of the SM's 16 a clock): both pipes
-// are full at once at best.
+// are full at once at best, 2048 clocks for both groups.  Measured 3300: a group's chain of load
+// (95 clocks), maximum (320), exponentials (1430), store and arrival (150), then its products, is
+// longer than twice the tensor time.  2048 new tokens over 16384 keys, 32 query heads on 8 of 128:
+// 474 us = 1086 TFLOP/s (256 blocks on 148 SMs: two rounds where 1.73 have work).  Every fourth
+// pair of exponentials as a polynomial on the FMA pipes: 545 us, not kept.
 //   warp 0     TMA: a page's part of a tile is one box per 64 dimensions (page sizes that
 //              divide 128 or are multiples of it), so a tile arrives swizzled whatever its pages
 //   warp 1     issues the products

@@ -33,7 +33,9 @@ __device__ __forceinline__ void grid_launch_dependents() {
 // ---------------------------------------------------------------------------
 // Row quantizer.  Bound: memory (x read once, q and the scales written once).  One block
 // per row; the row stays in registers, as it was read, between its absmax and its rounding
-// (32 values a thread, 8192 a row); longer rows are read again, from L1 or L2.
+// (32 values a thread, 8192 a row); longer rows are read again, from L1 or L2.  16384 x 8192: bf16
+// 76 us (5.3 TB/s), f32 97 us (6.9 TB/s).  (A block looping over rows with the next one read
+// ahead: 86 us for bf16: its registers leave four blocks on an SM instead of six.)
 // ---------------------------------------------------------------------------
 // The low bytes of four integers.
 __device__ __forceinline__ uint32_t pack_i8(int32_t a, int32_t b, int32_t c, int32_t d) {
@@ -171,6 +173,8 @@ void quantize(const void* x, int64_t rows, int64_t k, int64_t ldx, int8_t* q, in
 // product, which is what held the single-CTA form at 0.6 of the rate (128 x 256 x 32 moves
 // 96 bytes a clock in and 96 out, of 128).  For few rows it is the stream of W: rows of A past
 // m are filled with zeros without traffic, and narrow tiles spread W over all SMs.
+// Measured alone: 16384 x 8192 x 8192 660 us = 3330 TOPS, 4096 x 8192 x 8192 163 us = 3380 (tensor
+// pipe 91 % active); 2048 x 4096 x 14336 + GELU to f16 about 88 us.
 //   warp 0      TMA producer of its own CTA's operands, completing on the even CTA's barrier
 //   warp 1      of the even CTA: issues the products for both
 //   warps 2-9   epilogue: scale, bias, activation, rounding, a 64-byte-wide tile staged in
