@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const AttnParams P) {
   uint8_t* ring = smem + S::kQ;
   int64_t* offs = reinterpret_cast<int64_t*>(ring + kStages * S::kStage);  // [kStages + 1][KT], -1: zeros
 
+  grid_dependency_wait();
   grid_launch_dependents();
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int kv = a.kv_len[b];
@@ -332,9 +333,10 @@ __global__ void __launch_bounds__(256) k_attn_join(const JoinParams J) {
   const rg_paged_attention_args& a = P.p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hk = blockIdx.y, b = blockIdx.z, group = P.group.d;
   const int row = blockIdx.x * (8 / W) + warp / W, w = warp % W;
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int kv = a.kv_len[b];
-  grid_dependency_wait();
   if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) return;
   const int ql = (int)(q1 - q0), rows = ql * group;
   if (row >= rows) return;
@@ -399,7 +401,7 @@ rg_status go(const AttnParams& A, cudaStream_t st) {
   const int64_t tiles = (rows + S::kRows - 1) / S::kRows;
   if (tiles * A.splits > INT_MAX) return RG_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)(tiles * A.splits), (unsigned)A.p.c.kv_heads, (unsigned)A.p.a.batch);
-  kernel<<<grid, S::kThreads, S::kSmem, st>>>(A);
+  launch_early(kernel, grid, S::kThreads, S::kSmem, st, A);
   return RG_OK;
 }
 
@@ -429,20 +431,12 @@ rg_status launch_few(const AttnParams& A, cudaStream_t st) {
 
 template <typename T, int W>
 void launch_join(const JoinParams& J, int64_t rows, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((rows * W + 7) / 8), (unsigned)J.A.p.c.kv_heads, (unsigned)J.A.p.a.batch);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  const dim3 grid((unsigned)((rows * W + 7) / 8), (unsigned)J.A.p.c.kv_heads, (unsigned)J.A.p.a.batch);
   switch (J.A.p.c.head_dim) {
-    case 64: cudaLaunchKernelEx(&cfg, k_attn_join<T, 64, W>, J); break;
-    case 96: cudaLaunchKernelEx(&cfg, k_attn_join<T, 96, W>, J); break;
-    case 128: cudaLaunchKernelEx(&cfg, k_attn_join<T, 128, W>, J); break;
-    default: cudaLaunchKernelEx(&cfg, k_attn_join<T, 256, W>, J); break;
+    case 64: launch_early(k_attn_join<T, 64, W>, grid, 256, 0, st, J); break;
+    case 96: launch_early(k_attn_join<T, 96, W>, grid, 256, 0, st, J); break;
+    case 128: launch_early(k_attn_join<T, 128, W>, grid, 256, 0, st, J); break;
+    default: launch_early(k_attn_join<T, 256, W>, grid, 256, 0, st, J); break;
   }
 }
 template <typename T>

@@ -70,6 +70,9 @@ struct TcParams {
   uint32_t flip;          // sign bits to flip in a pair of Q's values
   uint64_t wait_ns;
   int32_t starve;
+  // The launch before is the kernel for few rows, which this one does not depend on: it waits
+  // for it at its end only.  (That kernel started after whatever ran before the call was over.)
+  int32_t beside;
 };
 
 // Instruction descriptor of tcgen05.mma kind::f16: f32 sums, A and B of one 16-bit type, B
@@ -125,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const rg_paged_attention_args& a = p.P.p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hk = blockIdx.y, b = blockIdx.z, group = (int)p.P.group.d;
+  if (!p.beside) grid_dependency_wait();
   grid_launch_dependents();
 
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
@@ -489,17 +493,9 @@ rg_status go(const AttnParams& P, bool beside, cudaStream_t st) {
   if (!cache_map<T>(&mk, c.k, c, p.box) || !cache_map<T>(&mv, c.v, c, p.box)) return RG_ERR_CUDA;
   const int64_t rows = (int64_t)P.p.a.max_q_len * P.group.d, blocks = (rows + kTcRows - 1) / kTcRows * P.splits;
   if (blocks > INT_MAX) return RG_ERR_UNSUPPORTED;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)P.p.a.batch);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = beside ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, mk, mv, p);
+  p.beside = beside;
+  const dim3 grid((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)P.p.a.batch);
+  launch_early(kernel, grid, kThreads, C::kSmem, st, mk, mv, p);
   return RG_OK;
 }
 

@@ -22,14 +22,6 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 
-// Waits for the launch before this one (and for its writes) when this launch was allowed to
-// start beside it; else returns at once.
-__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the launch after this one start, if it is allowed to.
-__device__ __forceinline__ void grid_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 // ---------------------------------------------------------------------------
 // Row quantizer.  Bound: memory (x read once, q and the scales written once).  One block
 // per row; the row stays in registers, as it was read, between its absmax and its rounding
@@ -88,6 +80,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 6 : 4)
     }
   };
   __shared__ float red[kQuantThreads / 32];
+  grid_dependency_wait();
   grid_launch_dependents();
   const int chunks = (int)(ldq / E);
   const auto read = [&](int64_t r, int c) {
@@ -159,8 +152,9 @@ void quantize(const void* x, int64_t rows, int64_t k, int64_t ldx, int8_t* q, in
               cudaStream_t st) {
   const bool vec = (((uintptr_t)x | (uintptr_t)(ldx * (int64_t)sizeof(T))) & 15) == 0;
   const T* p = static_cast<const T*>(x);
-  if (vec) k_quantize_token<T, true><<<(unsigned)rows, kQuantThreads, 0, st>>>(p, k, ldx, q, ldq, scale);
-  else k_quantize_token<T, false><<<(unsigned)rows, kQuantThreads, 0, st>>>(p, k, ldx, q, ldq, scale);
+  const dim3 grid((unsigned)rows);
+  if (vec) launch_early(k_quantize_token<T, true>, grid, kQuantThreads, 0, st, p, k, ldx, q, ldq, scale);
+  else launch_early(k_quantize_token<T, false>, grid, kQuantThreads, 0, st, p, k, ldx, q, ldq, scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -341,6 +335,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1)
     uint32_t phase = 0;
     bool ok = true;
     int issued = 0;
+    if (!p.g.after_quantizer) grid_dependency_wait();  // else only what the quantizer writes is waited for
     for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
       int mb, nb;
       pair_tile(tile, p, mb, nb);
@@ -570,6 +565,7 @@ __global__ void __launch_bounds__(kFewThreads)
 
   if (warp == 0) {
     if (!p.starve) {
+      if (!g.after_quantizer) grid_dependency_wait();  // else only what the quantizer writes is waited for
       const uint32_t ring = smem_addr(smem);
       const uint32_t bytes = (uint32_t)(128 + p.box_rows) * kBK;
       const int first = min(p.stages, kb1 - kb0);
@@ -769,6 +765,8 @@ __global__ void __launch_bounds__(kSkinnyThreads, 3) k_linear_skinny(const Skinn
   };
   uint4 w0[U], w1[U];
   const int tile = blockIdx.x;
+  grid_dependency_wait();
+  grid_launch_dependents();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     w0[u] = load_w((int64_t)tile * 16 + gr, warp + u * kSkinnyWarps);
@@ -876,7 +874,7 @@ rg_status go_skinny(const TokenGemmArgs& a, const void* x, int64_t k, int64_t ld
   p.m = (int32_t)a.m;
   p.pitch = (int32_t)a.ld + 16;
   p.vec = (((uintptr_t)x | (uintptr_t)(ldx * (int64_t)sizeof(TX))) & 15) == 0;
-  k_linear_skinny<TX, TO><<<(unsigned)((a.n + 15) / 16), kSkinnyThreads, p.m * p.pitch, st>>>(p);
+  launch_early(k_linear_skinny<TX, TO>, dim3((unsigned)((a.n + 15) / 16)), kSkinnyThreads, p.m * p.pitch, st, p);
   return RG_OK;
 }
 
@@ -932,17 +930,7 @@ rg_status go_pair(const TokenGemmArgs& a, cudaStream_t st) {
   p.wait_ns = a.wait_ns ? a.wait_ns : kWaitNs;
   p.starve = a.starve;
   const int pairs = (int)std::min<int64_t>(tm * tn, 74);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * pairs);
-  cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = kGemmSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.after_quantizer ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, ma, mw, mo, p);
+  launch_early(kernel, dim3(2 * pairs), kGemmThreads, kGemmSmem, st, ma, mw, mo, p);
   return RG_OK;
 }
 
@@ -987,11 +975,9 @@ rg_status go_few(const TokenGemmArgs& a, int32_t tokens, cudaStream_t st) {
     attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
     ++na;
   }
-  if (a.after_quantizer) {
-    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[na].val.programmaticStreamSerializationAllowed = 1;
-    ++na;
-  }
+  attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[na].val.programmaticStreamSerializationAllowed = 1;
+  ++na;
   cfg.attrs = attr;
   cfg.numAttrs = na;
   cudaLaunchKernelEx(&cfg, kernel, mw, ma, p);

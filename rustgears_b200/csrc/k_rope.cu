@@ -29,6 +29,8 @@ __global__ void __launch_bounds__(kThreads)
     k_rope(const RopeArgs a, int32_t tokens_per_block, FastDiv per_token, FastDiv units, FastDiv page_size) {
   // units: work items of one head (rot / 2P rotations, then (head_dim - rot) / 2P copies);
   // per_token: those of all heads
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int i = blockIdx.y * kThreads + threadIdx.x;
   const int within = (int)per_token.div((uint32_t)i);
   if (within >= tokens_per_block) return;
@@ -142,8 +144,8 @@ rg_status go(const RopeArgs& a, cudaStream_t st) {
   if (blocks > INT_MAX) return RG_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)blocks, (unsigned)((tpb * per_token + kThreads - 1) / kThreads));
   const FastDiv by_token((uint32_t)per_token), by_head((uint32_t)units), by_page((uint32_t)a.page_size);
-  if (a.interleaved) k_rope<TI, TO, P, true><<<grid, kThreads, 0, st>>>(a, tpb, by_token, by_head, by_page);
-  else k_rope<TI, TO, P, false><<<grid, kThreads, 0, st>>>(a, tpb, by_token, by_head, by_page);
+  if (a.interleaved) launch_early(k_rope<TI, TO, P, true>, grid, kThreads, 0, st, a, tpb, by_token, by_head, by_page);
+  else launch_early(k_rope<TI, TO, P, false>, grid, kThreads, 0, st, a, tpb, by_token, by_head, by_page);
   return RG_OK;
 }
 

@@ -45,15 +45,7 @@ struct JoinParams {
 // powers of two, or multiples of 128.
 bool attention_tc_takes(const PagedAttnArgs& p);
 constexpr int kTcRows = 256, kTcKeys = 128;  // its tiles
-// `beside`: the launch may run beside the one before it (which it does not depend on).
+// `beside`: the launch before it is the kernel for few rows, which it does not depend on.
 rg_status launch_attention_tc(const AttnParams& P, bool beside, cudaStream_t st);
-
-// Waits for the launch before this one (and for its writes) when this launch was allowed to
-// start beside it; else returns at once.
-__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the launch after this one start, if it is allowed to.
-__device__ __forceinline__ void grid_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 
 }  // namespace rg

@@ -7,10 +7,36 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <utility>
 
 #include "../../include/rg_npu.h"
 
 namespace rg {
+
+// The serving kernels are launched so that each may start while the launch before it ends: its
+// blocks are placed and set up early, then wait.  Every kernel begins with grid_dependency_wait
+// (before it reads or writes anything another launch may have written or read) and lets the next
+// one start only after it, so that whatever ran earlier in the stream is over by then too.
+template <typename... P, typename... A>
+inline void launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+// Waits for the launch before this one and for its writes.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the launch after this one start.
+__device__ __forceinline__ void grid_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 // Runs a kernel's set-up once on every device (a function attribute belongs to the device
 // that was current).

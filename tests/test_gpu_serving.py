@@ -177,6 +177,73 @@ def test_linear_wider_weight_rows(gpu, sv):
     same(torch, got, rounded(torch, linear_reference(x, wq, sw, None, 0), "f32"))
 
 
+def test_calls_see_what_ran_just_before(gpu, sv):
+    """Launches start early but read nothing before their predecessors are over: inputs, weights,
+    lengths and caches rewritten right before each call, on one stream, eagerly and in a graph,
+    and from another stream through an event."""
+    torch = gpu
+    n, h, d = 64, 4, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    table = sv.rope_table(512, d)
+    kc, vc = (torch.zeros(8, 64, h, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    slots = torch.arange(n, device="cuda") + 64
+    bt = torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    data = [(torch.randn(n, 512, device="cuda", generator=g), torch.randn(3 * h * d, 512, device="cuda", generator=g))
+            for _ in range(6)]
+    x, w = torch.empty_like(data[0][0]), torch.empty_like(data[0][1])
+    big = torch.zeros(1 << 26, device="cuda")
+    kv_len = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def chain():
+        kv_len.fill_(n)
+        q, s = sv.quantize_weight_i8(w)
+        y = sv.linear_i8_token(x, q, s, out_dtype=torch.float16).view(n, 3 * h, d)
+        q = sv.kv_append(y[:, h:2 * h], y[:, 2 * h:], kc, vc, slots, positions=pos, table=table, q=y[:, :h])
+        o = sv.attention_paged(q, kc, vc, bt, kv_len, cu, max_q_len=n, max_kv_len=n)
+        one = sv.attention_paged(q[-1:], kc, vc, bt, kv_len, cu[:2] // n, max_q_len=1, max_kv_len=n)
+        kc.zero_()
+        vc.zero_()
+        kv_len.zero_()
+        return torch.cat([o, one])
+
+    def load(i):
+        big.add_(1.0)             # long enough that the launches behind it queue up
+        x.copy_(data[i][0])
+        w.copy_(data[i][1])
+
+    want = []
+    for i in range(6):
+        load(i)
+        torch.cuda.synchronize()
+        want.append(chain())
+        torch.cuda.synchronize()
+    got = []
+    for i in range(6):
+        load(i)
+        got.append(chain())
+    for a, b in zip(got, want):
+        same(torch, a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain()
+    side = torch.cuda.Stream()
+    for i in range(6):
+        ready = torch.cuda.Event()
+        with torch.cuda.stream(side):
+            load(i)
+            ready.record()
+        torch.cuda.current_stream().wait_event(ready)
+        if i % 2:
+            graph.replay()
+            copy = out.clone()
+        else:
+            copy = chain()
+        side.wait_stream(torch.cuda.current_stream())
+        same(torch, copy, want[i])
+
+
 def test_linear_kernel_level_calls(gpu, sv):
     """Quantizer and product called apart, the output a column block of a wider tensor."""
     torch, L = gpu, _native.lib()
