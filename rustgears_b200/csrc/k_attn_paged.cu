@@ -514,7 +514,9 @@ rg_status make_plan(const PagedAttnArgs& p, Plan& L) {
   if (L.few) {
     // (beside chunks: taken as one block for every other sequence)
     const int64_t blocks = L.many ? (seqs + 1) / 2 : seqs * ((L.rows + L.few_shape.rows - 1) / L.few_shape.rows);
-    const Pace pace = {296, 2.5, d <= 64 ? 0.6 : d <= 96 ? 0.8 : 1.1};
+    // blocks an SM holds at once (Shape::kSmem)
+    const int keys = L.few_shape.keys, smem = (L.few_shape.rows + 6 * keys) * (2 * d + 16) + 4 * keys * 8;
+    const Pace pace = {148 * std::min(3, 227 * 1024 / smem), 2.5, d <= 64 ? 0.6 : d <= 96 ? 0.8 : 1.1};
     L.few_shape.splits = split_keys(blocks, (p.a.max_kv_len + L.few_shape.keys - 1) / L.few_shape.keys,
                                     p.a.batch == 1, pace, 2, row_us);
   }
