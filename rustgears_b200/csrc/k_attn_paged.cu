@@ -37,9 +37,11 @@ using namespace mma16;
 constexpr int kStages = 3;
 constexpr float kLog2e = 1.44269504088896340736f;
 
+constexpr int few_keys(int d) { return d <= 128 ? 64 : 32; }
+
 template <int D, int WR, int WK>
 struct Shape {
-  static constexpr int KT = D <= 128 ? 64 : 32;    // keys of a tile: two blocks' rings fit an SM
+  static constexpr int KT = few_keys(D);           // keys of a tile: two blocks' rings fit an SM
   static constexpr int kWarps = WR * WK, kThreads = 32 * kWarps, kRows = 16 * WR;
   static constexpr int kKeys = KT / WK;            // keys of a warp in a tile
   static constexpr int kPitch = D * 2 + 16;        // odd multiple of 16 bytes: ldmatrix without conflicts
@@ -478,8 +480,9 @@ int split_keys(int64_t blocks, int64_t tiles, bool one_sequence, const Pace& pac
 }
 
 // Up to so many rows (tokens times the heads that share a key head) a sequence takes the kernel
-// for few rows.
-constexpr int kFewRows = 64;
+// for few rows: one block's; beside chunks one fragment's, so that a sequence of the batch costs
+// one block of that launch and not four of which three find nothing.
+constexpr int kFewRows = 64, kFewRowsBeside = 16;
 
 struct Plan {
   AttnParams A;
@@ -505,11 +508,11 @@ rg_status make_plan(const PagedAttnArgs& p, Plan& L) {
   L.many = L.rows > kFewRows && attention_tc_takes(p);
   L.few = !L.many || (p.a.batch > 1 && p.a.tokens < (int64_t)p.a.batch * p.a.max_q_len);
   A.min_rows = 0;
-  A.max_rows = L.many ? kFewRows : INT_MAX;
+  A.max_rows = L.many ? kFewRowsBeside : INT_MAX;
   const int d = p.c.head_dim;
   const double row_us = 8.0 * d * (double)p.a.tokens * p.a.heads / 5e6;  // partial rows written and read
   const int64_t seqs = (int64_t)p.c.kv_heads * p.a.batch;
-  L.few_shape = {few_rows(A), d <= 128 ? 64 : 32, 1};
+  L.few_shape = {few_rows(A), few_keys(d), 1};
   L.many_shape = {kTcRows, kTcKeys, 1};
   if (L.few) {
     // (beside chunks: taken as one block for every other sequence)
@@ -555,7 +558,7 @@ rg_status launch_attention_paged(const PagedAttnArgs& p, cudaStream_t st) {
   }
   if (L.many) {
     A.splits = L.many_shape.splits;
-    A.min_rows = L.few ? kFewRows : 0;
+    A.min_rows = L.few ? kFewRowsBeside : 0;
     A.max_rows = INT_MAX;
     s = launch_attention_tc(A, L.few, st);
     if (s != RG_OK) return s;
@@ -565,9 +568,11 @@ rg_status launch_attention_paged(const PagedAttnArgs& p, cudaStream_t st) {
     J.A = A;
     J.few = L.few_shape;
     J.many = L.many_shape;
-    J.limit = !L.many ? INT_MAX : L.few ? kFewRows : 0;
-    if (p.c.dtype == RG_DTYPE_F16) launch_join<__half>(J, L.rows, st);
-    else launch_join<__nv_bfloat16>(J, L.rows, st);
+    J.limit = !L.many ? INT_MAX : L.few ? kFewRowsBeside : 0;
+    // unsplit chunks have nothing to join: then the rows of the others only
+    const int64_t rows = L.many && L.many_shape.splits == 1 ? std::min<int64_t>(L.rows, J.limit) : L.rows;
+    if (p.c.dtype == RG_DTYPE_F16) launch_join<__half>(J, rows, st);
+    else launch_join<__nv_bfloat16>(J, rows, st);
   }
   return RG_OK;
 }
