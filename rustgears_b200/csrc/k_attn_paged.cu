@@ -20,8 +20,8 @@
 // cluster start together, which costs a wait for 16 free places; 16.2 against 11.3 us at one
 // token over 4001 keys.)
 //
-// Measured (32 query heads on 8 of 128, bf16): one token over 4001 keys 11.3 us (16.4 MB, half of
-// it launches and the join); over 131072 keys 95 us (5.6 TB/s); 64 sequences of up to 6144 keys
+// Measured (32 query heads on 8 of 128, bf16): one token over 4001 keys 11.2 us (16.4 MB, half of
+// it launches and the join); over 131072 keys 94 us (5.7 TB/s); 64 sequences of up to 6144 keys
 // 183 us (5.6 TB/s).
 #include <algorithm>
 #include <climits>
@@ -74,7 +74,6 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const AttnParams P) {
   int64_t* offs = reinterpret_cast<int64_t*>(ring + kStages * S::kStage);  // [kStages + 1][KT], -1: zeros
 
   grid_dependency_wait();
-  grid_launch_dependents();
   const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int kv = a.kv_len[b];
   if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) {
@@ -252,6 +251,8 @@ __global__ void __launch_bounds__(32 * WR * WK) k_attn_few(const AttnParams P) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
   }
+
+  grid_launch_dependents();  // (earlier, the next launch's blocks would sit unevenly among these)
 
   // ---- join the key groups: every warp scales to the rows' common maximum, adds in order ----
   cp_async_wait<0>();

@@ -19,7 +19,7 @@
 // are full at once at best, 2048 clocks for both groups.  Measured 3300: a group's chain of load
 // (95 clocks), maximum (320), exponentials (1430), store and arrival (150), then its products, is
 // longer than twice the tensor time.  2048 new tokens over 16384 keys, 32 query heads on 8 of 128:
-// 474 us = 1086 TFLOP/s (256 blocks on 148 SMs: two rounds where 1.73 have work).  Every fourth
+// 479 us = 1076 TFLOP/s (256 blocks on 148 SMs: two rounds where 1.73 have work).  Every fourth
 // pair of exponentials as a polynomial on the FMA pipes: 545 us, not kept.
 //   warp 0     TMA: a page's part of a tile is one box per 64 dimensions (page sizes that
 //              divide 128 or are multiples of it), so a tile arrives swizzled whatever its pages

@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1)
     const TokenGemmArgs& g = p.g;
     int iter = 0, turn = 0;
     grid_dependency_wait();  // the row scales come from the quantizer
+    grid_launch_dependents();
     for (int tile = pair; tile < num_tiles; tile += pairs, ++iter) {
       int mb, nb;
       pair_tile(tile, p, mb, nb);
@@ -616,8 +617,9 @@ __global__ void __launch_bounds__(kFewThreads)
     tc_fence_after();
     const int row = (warp & 3) * 32 + lane;  // of the tile: this thread's TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)(row & ~31) << 16);
+    grid_dependency_wait();  // the row scales come from the quantizer
+    grid_launch_dependents();
     if (p.splits == 1) {
-      grid_dependency_wait();  // the row scales come from the quantizer
       const int64_t n = n0 + row;
       const bool row_ok = n < g.n;
       const float sw = row_ok ? __ldg(g.w_scale + n) : 0.0f;
@@ -766,7 +768,6 @@ __global__ void __launch_bounds__(kSkinnyThreads, 3) k_linear_skinny(const Skinn
   uint4 w0[U], w1[U];
   const int tile = blockIdx.x;
   grid_dependency_wait();
-  grid_launch_dependents();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     w0[u] = load_w((int64_t)tile * 16 + gr, warp + u * kSkinnyWarps);
@@ -843,6 +844,9 @@ __global__ void __launch_bounds__(kSkinnyThreads, 3) k_linear_skinny(const Skinn
         }
       }
     }
+    // Not before: blocks of a launch placed among these would sit unevenly on the SMs (one token
+    // through 4096 -> 4096 back to back: 11.1 us with the trigger at the start, 8.3 here).
+    grid_launch_dependents();
     // d: rows gr and gr + 8, tokens 2 t4 and 2 t4 + 1
     *reinterpret_cast<int2*>(&part[warp][gr][2 * t4]) = make_int2(d[0], d[1]);
     *reinterpret_cast<int2*>(&part[warp][gr + 8][2 * t4]) = make_int2(d[2], d[3]);

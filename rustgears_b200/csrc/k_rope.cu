@@ -13,8 +13,8 @@
 // each of two places (half layout) or 2 P consecutive ones, P elements filling a 16-byte
 // access, so a warp's accesses are whole 128-byte lines; resident threads, not unrolling,
 // keep the loads in flight.  Measured: 16384 tokens x 32 heads of 128, f32, 64 dimensions rotated
-// 87 us (6.2 TB/s of 541 MB); append of 8192 tokens, 16 heads of 64, f32 to f16 28.8 us (5.3 TB/s);
-// 64 tokens 2.4 us, one token 2.0 us (a launch).
+// 87 us (6.2 TB/s of 541 MB); append of 8192 tokens, 16 heads of 64, f32 to f16 27.5 us (5.5 TB/s);
+// 64 tokens 2.2 us, one token 1.8 us (a launch).
 #include <climits>
 
 #include "rg_serving.h"

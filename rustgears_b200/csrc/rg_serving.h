@@ -16,7 +16,9 @@ namespace rg {
 // The serving kernels are launched so that each may start while the launch before it ends: its
 // blocks are placed and set up early, then wait.  Every kernel begins with grid_dependency_wait
 // (before it reads or writes anything another launch may have written or read) and lets the next
-// one start only after it, so that whatever ran earlier in the stream is over by then too.
+// one start only after it, so that whatever ran earlier in the stream is over by then too.  (The
+// product that follows its own quantizer reads W before it waits, and the chunk kernel beside the
+// one for few rows waits at its end: see there.)
 template <typename... P, typename... A>
 inline void launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A&&... args) {
   cudaLaunchConfig_t cfg = {};
