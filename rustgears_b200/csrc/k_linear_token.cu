@@ -496,13 +496,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Product for few tokens: the roles turned, so that a tile is 128 rows of W by up to 256
+// Product for few tokens: the roles turned, so that a tile is 128 rows of W by all the
 // tokens, and K split over a cluster of `splits` CTAs.
 //
-// Bound: the stream of W.  A pair's 64-column tile takes 4 KB of W per copy and per four
-// products, and neither a copy (about 250 clocks of its issuing thread) nor a product (about
-// 100 clocks, however narrow) gets cheaper with it: 0.33 us per 128 bytes of K, 17.6 us at
-// 64 x 4096 x 4096.  Here a copy brings 16 KB of W.  The splits' i32 sums are exact in any
+// Bound: the stream of W, then latency.  A pair's 64-column tile takes 4 KB of W per copy and
+// walks all of K: 16.0 us at 64 x 4096 x 4096, 12.5 here, where a copy brings 16 KB of W and the
+// splits share K.  The splits' i32 sums are exact in any
 // order; they meet in distributed shared memory, where CTA r of the cluster adds and
 // finishes its share of the tokens, four of W's rows a thread: a token's outputs are neighbours.
 //   warp 0  TMA producer: W (before the quantizer is done), then the tokens
@@ -513,7 +512,7 @@ constexpr int kFewThreads = 192, kFewStages = 12;
 
 struct FewParams {
   TokenGemmArgs g;
-  int32_t splits, num_kb, tokens;  // tokens of a tile
+  int32_t splits, num_kb;
   int32_t box_rows, n_cols, stages, stage_bytes, ring, tmem_cols;
   int32_t vec_out;  // four neighbouring outputs may be written at once
   uint64_t wait_ns;
@@ -543,8 +542,8 @@ __global__ void __launch_bounds__(kFewThreads)
   const TokenGemmArgs& g = p.g;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % p.splits;
-  const int64_t n0 = (int64_t)(blockIdx.x / p.splits) * 128, t0 = (int64_t)blockIdx.y * p.tokens;
-  const int tokens = (int)min((int64_t)p.tokens, g.m - t0);
+  const int64_t n0 = (int64_t)(blockIdx.x / p.splits) * 128;
+  const int tokens = (int)g.m;
   const int kb0 = (int)((int64_t)p.num_kb * split / p.splits), kb1 = (int)((int64_t)p.num_kb * (split + 1) / p.splits);
 
   if (threadIdx.x == 0) {
@@ -576,7 +575,7 @@ __global__ void __launch_bounds__(kFewThreads)
       }
       grid_dependency_wait();
       for (int s = 0; s < first; ++s)
-        tma_load_2d_elect(ring + s * p.stage_bytes + 128 * kBK, &map_a, &full[s], (kb0 + s) * kBK, (int)t0);
+        tma_load_2d_elect(ring + s * p.stage_bytes + 128 * kBK, &map_a, &full[s], (kb0 + s) * kBK, 0);
       int stage = 0;
       uint32_t phase = 0;  // of the use before: its product empties the stage
       for (int kb = kb0 + first; kb < kb1; ++kb) {
@@ -584,7 +583,7 @@ __global__ void __launch_bounds__(kFewThreads)
         const uint32_t sw = ring + stage * p.stage_bytes;
         expect_tx_elect(&full[stage], bytes);
         tma_load_2d_elect(sw, &map_w, &full[stage], kb * kBK, (int)n0);
-        tma_load_2d_elect(sw + 128 * kBK, &map_a, &full[stage], kb * kBK, (int)t0);
+        tma_load_2d_elect(sw + 128 * kBK, &map_a, &full[stage], kb * kBK, 0);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
       // Drain: a copy still on its way (after a wait gave up) lands before the CTA leaves.
@@ -632,11 +631,11 @@ __global__ void __launch_bounds__(kFewThreads)
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          y[j] = dequant((int32_t)v[j], __fmul_rn(t + j < tokens ? __ldg(g.a_scale + t0 + t + j) : 0.0f, sw), bi);
+          y[j] = dequant((int32_t)v[j], __fmul_rn(t + j < tokens ? __ldg(g.a_scale + t + j) : 0.0f, sw), bi);
         activate<T, 8>(y, g.act, g.act_param);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (t + j < tokens && row_ok) static_cast<T*>(g.out)[(t0 + t + j) * g.ldo + n] = ElemOf<T>::from(y[j]);
+          if (t + j < tokens && row_ok) static_cast<T*>(g.out)[(t + j) * g.ldo + n] = ElemOf<T>::from(y[j]);
       }
     } else {
       int32_t* part = reinterpret_cast<int32_t*>(smem);  // [tokens][128], over the operands
@@ -692,7 +691,7 @@ __global__ void __launch_bounds__(kFewThreads)
       for (int u = 0; u < kItems; ++u) {
         const int i = i0 + u * kFewThreads;
         if (i - lane >= items) break;  // warp-uniform
-        const int64_t t = t0 + lo + min(i, items - 1) / 32;
+        const int64_t t = lo + min(i, items - 1) / 32;
         const float sa = __ldg(g.a_scale + t);
         float y[4] = {dequant(v[u].x, __fmul_rn(sa, sw[0]), bi[0]), dequant(v[u].y, __fmul_rn(sa, sw[1]), bi[1]),
                       dequant(v[u].z, __fmul_rn(sa, sw[2]), bi[2]), dequant(v[u].w, __fmul_rn(sa, sw[3]), bi[3])};
@@ -939,13 +938,13 @@ rg_status go_pair(const TokenGemmArgs& a, cudaStream_t st) {
 }
 
 template <typename T>
-rg_status go_few(const TokenGemmArgs& a, int32_t tokens, cudaStream_t st) {
+rg_status go_few(const TokenGemmArgs& a, cudaStream_t st) {
+  const int tokens = (int)a.m;
   const auto kernel = k_gemm_token_few<T>;
   static DeviceOnce once;
   once.run([&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); });
   FewParams p;
   p.g = a;
-  p.tokens = tokens;
   p.box_rows = (tokens + 7) / 8 * 8;
   p.n_cols = (tokens + 15) / 16 * 16;
   p.tmem_cols = 32;
@@ -957,17 +956,17 @@ rg_status go_few(const TokenGemmArgs& a, int32_t tokens, cudaStream_t st) {
   p.stages = std::min(kFewStages, (tokens <= 64 ? 96 : 192) * 1024 / p.stage_bytes);
   p.ring = p.stages * p.stage_bytes + 1024;
   p.num_kb = (int32_t)((a.ld + kBK - 1) / kBK);
-  const int64_t tn = (a.n + 127) / 128, tm = (a.m + tokens - 1) / tokens;
+  const int64_t tn = (a.n + 127) / 128;
   p.splits = 1;  // as many as find an SM, each with two steps of K at least
-  while (p.splits < 8 && tn * tm * p.splits * 2 <= slots && p.num_kb >= p.splits * 4) p.splits *= 2;
-  if (tn * p.splits > INT_MAX || tm > 65535) return RG_ERR_UNSUPPORTED;
+  while (p.splits < 8 && tn * p.splits * 2 <= slots && p.num_kb >= p.splits * 4) p.splits *= 2;
+  if (tn * p.splits > INT_MAX) return RG_ERR_UNSUPPORTED;
   p.wait_ns = a.wait_ns ? a.wait_ns : kWaitNs;
   p.starve = a.starve;
   p.vec_out = (((uintptr_t)a.out | (uintptr_t)(a.ldo * (int64_t)sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
   CUtensorMap mw, ma;
   if (!operand_map(&mw, a.w, a.n, a.ld, 128) || !operand_map(&ma, a.a, a.m, a.ld, p.box_rows)) return RG_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tn * p.splits), (unsigned)tm);
+  cfg.gridDim = dim3((unsigned)(tn * p.splits));
   cfg.blockDim = dim3(kFewThreads);
   cfg.dynamicSmemBytes = 1024 + p.ring + 512;
   cfg.stream = st;
@@ -992,9 +991,9 @@ rg_status go_few(const TokenGemmArgs& a, int32_t tokens, cudaStream_t st) {
 // rounds over the 74 pairs times the tile's width.
 template <typename T>
 rg_status go_gemm(const TokenGemmArgs& a, cudaStream_t st) {
-  // Measured at 4096 x 4096: 10.3 against 17.6 us at 1 token, 13.7 / 17.5 at 64, 15.0 / 17.9 at 128,
-  // 19.8 / 18.4 at 256.
-  if (a.m <= 128) return go_few<T>(a, (int32_t)a.m, st);
+  // Few tokens against pairs, us: 10.1 / 15.7 at 17 x 4096 x 4096, 12.5 / 16.0 at 64, 14.6 / 17.3 at 128;
+  // 18.6 / 20.8 at 64 x 4096 x 14336, 24.6 / 22.2 at 128; 10.3 / 8.1 at 128 x 1024 x 1024.
+  if (a.m <= 96) return go_few<T>(a, st);
   const auto cost = [&](int64_t bn) { return ((a.m + 255) / 256 * ((a.n + bn - 1) / bn) + 73) / 74 * (bn + 96); };
   if (cost(256) <= cost(128) && cost(256) <= cost(64)) return go_pair<256, T>(a, st);
   return cost(128) <= cost(64) ? go_pair<128, T>(a, st) : go_pair<64, T>(a, st);
