@@ -611,8 +611,10 @@ __global__ void __launch_bounds__(kFewThreads)
     volatile int never = 0;  // all products have completed before TMEM is freed
     warp_wait(tfull, 0, &never, p.wait_ns + kDrainNs);
   } else {
-    const bool got = mbar_wait_tight(tfull, 0, abort, p.wait_ns);
-    if (!__all_sync(0xffffffffu, got)) *abort = 1;
+    // The warp's result, not the lane's: what follows it (tcgen05.ld, the activations' votes) takes
+    // whole warps.  After a give-up, here or of the products, there are no sums to read.
+    const bool got = __all_sync(0xffffffffu, mbar_wait_tight(tfull, 0, abort, p.wait_ns) && !*abort);
+    if (!got) *abort = 1;
     tc_fence_after();
     const int row = (warp & 3) * 32 + lane;  // of the tile: this thread's TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)(row & ~31) << 16);
@@ -640,7 +642,7 @@ __global__ void __launch_bounds__(kFewThreads)
     } else {
       int32_t* part = reinterpret_cast<int32_t*>(smem);  // [tokens][128], over the operands
 #pragma unroll 1
-      for (int t = 0; t < tokens; t += 8) {
+      for (int t = 0; t < tokens && got; t += 8) {
         uint32_t v[8];
         tmem_ld8(lanes + t, v);
         tmem_ld_wait();

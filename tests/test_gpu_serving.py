@@ -686,6 +686,25 @@ def test_linear_bounded_waits_are_reported(gpu, sv, m):
     same(torch, got, rounded(torch, linear_reference(x, wq, sw, b, 0), "f32"))
 
 
+@pytest.mark.parametrize("act,code", [("none", 0), ("gelu", 4)])
+@pytest.mark.parametrize("k", [256, 4096])
+def test_linear_few_tokens_leave_together(gpu, sv, k, act, code):
+    """9 to 96 tokens, K whole and split: a warp whose wait runs out leaves as one, also where the
+    f32 GELU votes inside the loop over the tokens."""
+    torch, L = gpu, _native.lib()
+    x, wq, sw, b = linear_case(50, k, 300, seed=2)
+    for wait in (1, 1000, 1000000):
+        try:
+            L.rg_debug_set_tc_wait(wait, 1)
+            run_linear(torch, sv, x, wq, sw, b, act, "f32", "f32")
+            with pytest.raises(_native.RgError, match="bounded wait"):
+                sv.check()
+        finally:
+            L.rg_debug_set_tc_wait(0, 0)
+    got = run_linear(torch, sv, x, wq, sw, b, act, "f32", "f32")
+    same(torch, got, rounded(torch, linear_reference(x, wq, sw, b, code), "f32"))
+
+
 def test_attention_bounded_waits_are_reported(gpu, sv):
     """Without loads the chunk kernel's waits run out: reported, and the next call is right."""
     torch, L = gpu, _native.lib()
