@@ -488,7 +488,7 @@ rg_status go(const AttnParams& P, bool beside, cudaStream_t st) {
   p.scale2 = fmaxf(fabsf(P.scale2), FLT_MIN);
   p.flip = P.scale2 < 0.0f ? 0x80008000u : 0u;
   p.wait_ns = P.p.wait_ns ? P.p.wait_ns : kWaitNs;
-  p.starve = P.p.starve;
+  p.starve = P.p.starve == 1;
   CUtensorMap mk, mv;
   if (!cache_map<T>(&mk, c.k, c, p.box) || !cache_map<T>(&mv, c.v, c, p.box)) return RG_ERR_CUDA;
   const int64_t rows = (int64_t)P.p.a.max_q_len * P.group.d, blocks = (rows + kTcRows - 1) / kTcRows * P.splits;

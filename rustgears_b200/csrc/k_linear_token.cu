@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kFewThreads)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
-    if (!p.starve) {
+    if (p.starve != 1) {
       if (!g.after_quantizer) grid_dependency_wait();  // else only what the quantizer writes is waited for
       const uint32_t ring = smem_addr(smem);
       const uint32_t bytes = (uint32_t)(128 + p.box_rows) * kBK;
@@ -576,9 +576,9 @@ __global__ void __launch_bounds__(kFewThreads)
       grid_dependency_wait();
       for (int s = 0; s < first; ++s)
         tma_load_2d_elect(ring + s * p.stage_bytes + 128 * kBK, &map_a, &full[s], (kb0 + s) * kBK, 0);
-      int stage = 0;
+      int stage = 0, issued = first;
       uint32_t phase = 0;  // of the use before: its product empties the stage
-      for (int kb = kb0 + first; kb < kb1; ++kb) {
+      for (int kb = kb0 + first; kb < kb1; ++kb, ++issued) {
         if (!warp_wait(&empty[stage], phase, abort, p.wait_ns)) break;
         const uint32_t sw = ring + stage * p.stage_bytes;
         expect_tx_elect(&full[stage], bytes);
@@ -586,18 +586,21 @@ __global__ void __launch_bounds__(kFewThreads)
         tma_load_2d_elect(sw + 128 * kBK, &map_a, &full[stage], kb * kBK, 0);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
-      // Drain: a copy still on its way (after a wait gave up) lands before the CTA leaves.
-      if (*abort) {
-        volatile int never = 0;
-        for (int s = 0; s < first; ++s) warp_wait(&full[s], s < stage ? phase ^ 1 : phase, &never, kDrainNs);
+      // Drain: every stage's last copies land before the CTA leaves, whoever gave up and when (after
+      // the last copy was issued, too).  Where nobody did, the products wait for them anyway.
+      volatile int never = 0;
+      for (int s = 0; s < first; ++s) {
+        const int op = issued - 1 - s;
+        warp_wait(&full[op % p.stages], (uint32_t)(op / p.stages) & 1, &never, kDrainNs);
       }
     }
   } else if (warp == 1) {
     const uint32_t idesc = idesc_i8(128, p.n_cols), ring = smem_addr(smem);
     int stage = 0;
     uint32_t phase = 0;
+    if (p.starve == 2) *abort = 1;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!warp_wait(&full[stage], phase, abort, p.wait_ns)) break;
+      if (p.starve == 2 || !warp_wait(&full[stage], phase, abort, p.wait_ns)) break;
       tc_fence_after();
       const uint32_t sw = ring + stage * p.stage_bytes;
       const uint64_t dw = desc_kmajor_sw128(sw), dx = desc_kmajor_sw128(sw + 128 * kBK);
@@ -933,7 +936,7 @@ rg_status go_pair(const TokenGemmArgs& a, cudaStream_t st) {
   p.num_kb = (int32_t)((a.ld + kBK - 1) / kBK);
   p.group_m = 16;
   p.wait_ns = a.wait_ns ? a.wait_ns : kWaitNs;
-  p.starve = a.starve;
+  p.starve = a.starve == 1;
   const int pairs = (int)std::min<int64_t>(tm * tn, 74);
   launch_early(kernel, dim3(2 * pairs), kGemmThreads, kGemmSmem, st, ma, mw, mo, p);
   return RG_OK;

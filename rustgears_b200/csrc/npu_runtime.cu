@@ -1036,7 +1036,7 @@ static rg_status run_gemm_q(Session& s, const Op& lin, const int8_t* q, int64_t 
   g.amax = sink;
   g.err = s.errw.as<int>();
   g.wait_ns = g_tc_wait_ns.load();
-  g.starve = g_tc_starve.load();
+  g.starve = g_tc_starve.load() == 1;
   const bool tc = gemm_tc_eligible(g);
   const bool narrow = !tc && gemm_narrow_eligible(g);
   if (tc) {
@@ -1415,7 +1415,7 @@ static rg_status execute(Session& s, const float* x_dev, const RunPlan& P, float
         GemmArgs g;
         g.err = s.errw.as<int>();
         g.wait_ns = g_tc_wait_ns.load();
-        g.starve = g_tc_starve.load();
+        g.starve = g_tc_starve.load() == 1;
         bool fused_q = false;
         // a calibrated Linear's frozen activation scale (device), else null
         const float* frozen = s.calibrated && s.calib_off[i] >= 0 ? s.d_calib.as<float>() + s.calib_off[i] : nullptr;
@@ -2548,7 +2548,7 @@ rg_status rg_gemm_i8_fused(const int8_t* a, const int8_t* w, int64_t m, int64_t 
   RG_CUDA_TRY(cudaMemsetAsync(slot.ptr, 0, sizeof(int32_t), st));
   g.err = slot.ptr;
   g.wait_ns = g_tc_wait_ns.load();
-  g.starve = g_tc_starve.load();
+  g.starve = g_tc_starve.load() == 1;
   if (!launch_gemm_tc(g, sms, st)) return fail(RG_ERR_CUDA, "TMA descriptor encoding failed");
   RG_CUDA_TRY(cudaGetLastError());
   if (cap != cudaStreamCaptureStatusNone) return RG_OK;
@@ -2568,7 +2568,7 @@ rg_status rg_status_from_error_words(const int32_t words[2]) {
 
 void rg_debug_set_tc_wait(uint64_t wait_ns, int32_t starve_loads) {
   g_tc_wait_ns.store(wait_ns);
-  g_tc_starve.store(starve_loads ? 1 : 0);
+  g_tc_starve.store(starve_loads == 2 ? 2 : starve_loads ? 1 : 0);
 }
 
 int64_t rg_linear_i8_workspace_size(int64_t m, int64_t ld) { return round_up(m * ld, 256) + 256; }

@@ -10,7 +10,7 @@ namespace rg {
 // Sets the calling thread's rg_last_error() message; returns st.
 rg_status set_last_error(rg_status st, const char* msg);
 // What rg_debug_set_tc_wait holds: the limit of the tcgen05 kernels' waits (0: the default)
-// and whether they are to issue no operand loads.
+// and what is made to fail: 1 no operand loads are issued, 2 the products are given up at once.
 void tc_wait_hook(uint64_t* wait_ns, int32_t* starve);
 
 // Where the absmax of an op's output goes (the next quantizing op's input scale).

@@ -139,7 +139,7 @@ struct TokenGemmArgs {
   int32_t* err = nullptr;
   uint64_t wait_ns = 0;  // limit of every pipeline wait (0: the default)
   int32_t after_quantizer = 0;  // a and a_scale come from the quantizer launched just before
-  int32_t starve = 0;    // test hook: issue no operand loads, so the waits run out
+  int32_t starve = 0;    // test hook: 1 issue no operand loads, so the waits run out; 2 give the products up at once
 };
 rg_status launch_gemm_token(const TokenGemmArgs& a, cudaStream_t st);
 // Quantizer and product in one launch for a few tokens (a, a_scale unused).

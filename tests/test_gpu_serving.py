@@ -705,6 +705,27 @@ def test_linear_few_tokens_leave_together(gpu, sv, k, act, code):
     same(torch, got, rounded(torch, linear_reference(x, wq, sw, b, code), "f32"))
 
 
+@pytest.mark.parametrize("m,k,n", [(64, 4096, 400), (40, 256, 400), (96, 9000, 300)])
+def test_linear_given_up_with_copies_on_their_way(gpu, sv, m, k, n):
+    """The products are given up while, or after, the last copies are issued: those land before
+    their blocks leave, the call is reported, and calls that take over their SMs are right."""
+    torch, L = gpu, _native.lib()
+    x, wq, sw, b = linear_case(m, k, n, seed=3)
+    want = rounded(torch, linear_reference(x, wq, sw, b, 0), "f32")
+    same(torch, run_linear(torch, sv, x, wq, sw, b, "none", "f32", "f32"), want)
+    for _ in range(3):
+        try:
+            L.rg_debug_set_tc_wait(1000000, 2)
+            run_linear(torch, sv, x, wq, sw, b, "none", "f32", "f32")
+        finally:
+            L.rg_debug_set_tc_wait(0, 0)
+        got = run_linear(torch, sv, x, wq, sw, b, "none", "f32", "f32")
+        with pytest.raises(_native.RgError, match="bounded wait") as e:
+            sv.check()
+        assert e.value.status == _native.RG_ERR_TIMEOUT
+        same(torch, got, want)
+
+
 def test_attention_bounded_waits_are_reported(gpu, sv):
     """Without loads the chunk kernel's waits run out: reported, and the next call is right."""
     torch, L = gpu, _native.lib()
