@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     int next = look(0);
     int op = 0;
-    bool ok = !p.starve;
+    bool ok = p.starve != 1;
     for (int n = 0; n < tiles && ok; ++n) {
       const int page = next;
       next = look(n + 1);
@@ -226,12 +226,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (*abort) {  // a copy still on its way lands before the CTA leaves
-      volatile int never = 0;
-      for (int s = 0; s < C::kStages && s < op; ++s) {
-        const int o = op - 1 - s;
-        warp_wait(&full[o % C::kStages], (o / C::kStages) & 1, &never, kDrainNs);
-      }
+    // Every stage's last copies land before the CTA leaves, whoever gave up and when (after the last
+    // copy was issued, too).  Where nobody did, the products wait for them anyway.
+    volatile int never = 0;
+    for (int s = 0; s < C::kStages && s < op; ++s) {
+      const int o = op - 1 - s;
+      warp_wait(&full[o % C::kStages], (o / C::kStages) & 1, &never, kDrainNs);
     }
   } else if (warp == 1) {
     // ---------------- products ----------------
@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_16_ss_elect(tmem + g * kTile, q + at, k + at, id_s, i != 0);
         }
       };
-      bool ok = warp_wait(q_ready, 0, abort, p.wait_ns) && wait_op(0);
+      if (p.starve == 2) *abort = 1;
+      bool ok = p.starve != 2 && warp_wait(q_ready, 0, abort, p.wait_ns) && wait_op(0);
       if (ok) {
         tc_fence_after();
         for (int g = 0; g < groups; ++g) {
@@ -488,7 +489,7 @@ rg_status go(const AttnParams& P, bool beside, cudaStream_t st) {
   p.scale2 = fmaxf(fabsf(P.scale2), FLT_MIN);
   p.flip = P.scale2 < 0.0f ? 0x80008000u : 0u;
   p.wait_ns = P.p.wait_ns ? P.p.wait_ns : kWaitNs;
-  p.starve = P.p.starve == 1;
+  p.starve = P.p.starve;
   CUtensorMap mk, mv;
   if (!cache_map<T>(&mk, c.k, c, p.box) || !cache_map<T>(&mv, c.v, c, p.box)) return RG_ERR_CUDA;
   const int64_t rows = (int64_t)P.p.a.max_q_len * P.group.d, blocks = (rows + kTcRows - 1) / kTcRows * P.splits;

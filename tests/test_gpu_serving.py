@@ -741,6 +741,29 @@ def test_attention_bounded_waits_are_reported(gpu, sv):
     check_attention(torch, sv, [(100, 300)], 4, 2, 64, torch.float16, 16, "token")
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("lens", [[(100, 300)], [(600, 5000)], [(300, 1500), (1, 700)]])
+def test_attention_given_up_with_copies_on_their_way(gpu, sv, dim, page, lens):
+    """The products of chunks are given up while, or after, the last copies are issued: those land
+    before their blocks leave, the call is reported, and the call that takes over their SMs is right."""
+    torch, L = gpu, _native.lib()
+    args = make_batch(torch, lens, 4, 2, dim, torch.bfloat16, page, "token")
+    most = dict(max_q_len=max(a for a, _ in lens), max_kv_len=max(b for _, b in lens))
+    want = sv.attention_paged(*args, **most)
+    for _ in range(3):
+        try:
+            L.rg_debug_set_tc_wait(1000000, 2)
+            sv.attention_paged(*args, **most)
+        finally:
+            L.rg_debug_set_tc_wait(0, 0)
+        got = sv.attention_paged(*args, **most)
+        with pytest.raises(_native.RgError, match="bounded wait") as e:
+            sv.check()
+        assert e.value.status == _native.RG_ERR_TIMEOUT
+        same(torch, got, want)
+    check_attention(torch, sv, lens, 4, 2, dim, torch.bfloat16, page, "token")
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 384])
 def test_attention_long_chunks(gpu, sv, dim, page):
