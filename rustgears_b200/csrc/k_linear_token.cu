@@ -65,8 +65,7 @@ struct AbsMax<__nv_bfloat16> {
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 6 : 4)
-    k_quantize_token(const T* __restrict__ x, int64_t k, int64_t ldx, int8_t* __restrict__ q,
-                     int64_t ldq, float* __restrict__ scale) {
+    k_quantize_token(const T* x, int64_t k, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
   constexpr int E = VEC ? 16 / (int)sizeof(T) : 4;  // values a thread handles at once
   constexpr int NREG = 32 / E;
   // A chunk as it was read: 32-bit words, taken apart where they are used (16-bit values would be
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1)
       int mb, nb;
       pair_tile(tile, p, mb, nb);
       const int64_t row0 = (int64_t)mb * 256 + rank * 128 + q * 32, row = row0 + lane;
-      const float sa = row < g.m ? __ldg(g.a_scale + row) : 0.0f;
+      const float sa = row < g.m ? g.a_scale[row] : 0.0f;
       const int buf = iter & 1;
       const bool got = mbar_wait_tight(&tfull[buf], (iter >> 1) & 1, abort, p.wait_ns);
       if (!__all_sync(0xffffffffu, got)) { *abort = 1; break; }
@@ -416,8 +415,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) __cluster_dims__(2, 1, 1)
         tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + c0), v);
         // lane j holds column col0 + j's scale and bias: one load each, broadcast by shuffles
         const bool in = col0 + lane < g.n;
-        const float sw = in ? __ldg(g.w_scale + col0 + lane) : 0.0f;
-        const float bi = in && g.bias ? __ldg(g.bias + col0 + lane) : 0.0f;
+        const float sw = in ? g.w_scale[col0 + lane] : 0.0f;
+        const float bi = in && g.bias ? g.bias[col0 + lane] : 0.0f;
         tmem_ld_wait();
         float y[32];
 #pragma unroll
@@ -626,8 +625,8 @@ __global__ void __launch_bounds__(kFewThreads)
     if (p.splits == 1) {
       const int64_t n = n0 + row;
       const bool row_ok = n < g.n;
-      const float sw = row_ok ? __ldg(g.w_scale + n) : 0.0f;
-      const float bi = row_ok && g.bias ? __ldg(g.bias + n) : 0.0f;
+      const float sw = row_ok ? g.w_scale[n] : 0.0f;
+      const float bi = row_ok && g.bias ? g.bias[n] : 0.0f;
 #pragma unroll 1
       for (int t = 0; t < tokens && got; t += 8) {
         uint32_t v[8];
@@ -636,7 +635,7 @@ __global__ void __launch_bounds__(kFewThreads)
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          y[j] = dequant((int32_t)v[j], __fmul_rn(t + j < tokens ? __ldg(g.a_scale + t + j) : 0.0f, sw), bi);
+          y[j] = dequant((int32_t)v[j], __fmul_rn(t + j < tokens ? g.a_scale[t + j] : 0.0f, sw), bi);
         activate<T, 8>(y, g.act, g.act_param);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -669,8 +668,8 @@ __global__ void __launch_bounds__(kFewThreads)
     float sw[4], bi[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      sw[j] = n + j < g.n ? __ldg(g.w_scale + n + j) : 0.0f;
-      bi[j] = n + j < g.n && g.bias ? __ldg(g.bias + n + j) : 0.0f;
+      sw[j] = n + j < g.n ? g.w_scale[n + j] : 0.0f;
+      bi[j] = n + j < g.n && g.bias ? g.bias[n + j] : 0.0f;
     }
     const bool whole = n + 4 <= g.n && p.vec_out;
 #pragma unroll 1
@@ -697,7 +696,7 @@ __global__ void __launch_bounds__(kFewThreads)
         const int i = i0 + u * kFewThreads;
         if (i - lane >= items) break;  // warp-uniform
         const int64_t t = lo + min(i, items - 1) / 32;
-        const float sa = __ldg(g.a_scale + t);
+        const float sa = g.a_scale[t];
         float y[4] = {dequant(v[u].x, __fmul_rn(sa, sw[0]), bi[0]), dequant(v[u].y, __fmul_rn(sa, sw[1]), bi[1]),
                       dequant(v[u].z, __fmul_rn(sa, sw[2]), bi[2]), dequant(v[u].w, __fmul_rn(sa, sw[3]), bi[3])};
         activate<T, 4>(y, g.act, g.act_param);
@@ -767,7 +766,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 3) k_linear_skinny(const Skinn
   const uint4 zero = make_uint4(0, 0, 0, 0);
   const auto load_w = [&](int64_t row, int s) {  // 16 bytes of a row at step s
     const int at = s * 64 + t4 * 16;
-    return row < g.n && at < ld ? __ldg(reinterpret_cast<const uint4*>(g.w + row * ld + at)) : zero;
+    return row < g.n && at < ld ? *reinterpret_cast<const uint4*>(g.w + row * ld + at) : zero;
   };
   uint4 w0[U], w1[U];
   const int tile = blockIdx.x;
@@ -862,7 +861,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 3) k_linear_skinny(const Skinn
         int32_t sum = 0;
 #pragma unroll
         for (int i = 0; i < kSkinnyWarps; ++i) sum += part[i][r][t];
-        const float y = dequant(sum, __fmul_rn(scales[t], __ldg(g.w_scale + n)), g.bias ? __ldg(g.bias + n) : 0.0f);
+        const float y = dequant(sum, __fmul_rn(scales[t], g.w_scale[n]), g.bias ? g.bias[n] : 0.0f);
         static_cast<TO*>(g.out)[t * g.ldo + n] =
             ElemOf<TO>::from(sizeof(TO) == 2 && (g.act == ACT_GELU || g.act == ACT_SILU)
                                  ? smooth16(g.act, y)

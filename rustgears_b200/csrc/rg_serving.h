@@ -19,6 +19,9 @@ namespace rg {
 // one start only after it, so that whatever ran earlier in the stream is over by then too.  (The
 // product that follows its own quantizer reads W before it waits, and the chunk kernel beside the
 // one for few rows waits at its end: see there.)
+// So a kernel's life begins while what it reads is still being written.  Its loads are therefore
+// plain ones: never the read-only path (__ldg, or const __restrict__ parameters), which promises
+// data that is constant for the whole launch and lets a load be moved above the wait.
 template <typename... P, typename... A>
 inline void launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A&&... args) {
   cudaLaunchConfig_t cfg = {};
