@@ -369,7 +369,10 @@ rg_status rg_gemm_i8_token(const int8_t* a, const float* a_scale, const int8_t* 
                            int32_t out_dtype, int64_t ldo, int32_t* error_words, void* stream);
 /* The two in one call: x [m, k] (row stride ldx) against w [n, ld], ld >= k.  `workspace`
  * holds rg_linear_i8_token_workspace_size(m, n, ld) bytes, 256-byte aligned (NULL when that is
- * 0), and is free again once the call's work on `stream` is done. */
+ * 0), and is free again once the call's work on `stream` is done.  Where that size is not 0, out
+ * may overlap x (all of x has been read when out is written); where it is 0 the call is one
+ * launch that reads x while it writes out, and an overlap is refused (the two calls above
+ * do the same in two launches). */
 typedef struct rg_linear_token_args {
   const void* x; const int8_t* w; const float* w_scale; const float* bias; void* out;
   int64_t m, k, ldx, n, ld, ldo;

@@ -198,6 +198,12 @@ at::Tensor rows_of(const at::Tensor& x) {
   return r;
 }
 int64_t ldx_of(const at::Tensor& r) { return r.size(0) > 1 ? r.stride(0) : r.size(1); }
+// Whether rows_of's rows and a contiguous tensor lie in overlapping ranges of memory.
+bool ranges_meet(const at::Tensor& r, const at::Tensor& out) {
+  const char *x = static_cast<const char*>(r.data_ptr()), *o = static_cast<const char*>(out.data_ptr());
+  const int64_t size = ((r.size(0) - 1) * ldx_of(r) + r.size(1)) * (int64_t)r.element_size();
+  return x < o + out.nbytes() && o < x + size;
+}
 
 // ---------------------------------------------------------------------------
 // the calls
@@ -258,6 +264,20 @@ PyObject* linear(PyObject* const* o) {
   at::Tensor out = given ? *given : empty(shape, type, dev.index);
   if (m > 0) {
     const int64_t need = rg_linear_i8_token_workspace_size(m, n, ld);
+    if (need == 0 && given && ranges_meet(r, out)) {
+      // one launch would write out while it reads x: quantized first, as larger calls do
+      at::Tensor q = empty({m, ld}, at::kChar, dev.index), s = empty({m}, at::kFloat, dev.index);
+      int32_t* words = error_words(dev.index);
+      call(dev.index, [&](void* st) {
+        const rg_status e = rg_quantize_token_i8(r.data_ptr(), dtype_code(r.scalar_type()), m, k, ldx_of(r),
+                                                 q.data_ptr<int8_t>(), ld, s.data_ptr<float>(), st);
+        if (e != RG_OK) return e;
+        return rg_gemm_i8_token(q.data_ptr<int8_t>(), s.data_ptr<float>(), w.data_ptr<int8_t>(), ws.data_ptr<float>(),
+                                m, n, ld, bias ? bias->data_ptr<float>() : nullptr, a.act, a.act_param, out.data_ptr(),
+                                code, n, words, st);
+      });
+      return THPVariable_Wrap(out);
+    }
     at::Tensor space;
     if (need > 0) space = empty({need}, at::kByte, dev.index);
     a.x = r.data_ptr();

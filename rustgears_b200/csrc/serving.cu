@@ -67,6 +67,19 @@ rg_status check_gemm(const char* f, const int8_t* w, const float* w_scale, int64
   return RG_OK;
 }
 
+// Whether any of m rows of `a` bytes, `as` bytes apart, shares memory with one of m rows of `b`
+// bytes, `bs` bytes apart (m is small).
+bool rows_overlap(const void* x, int64_t a, int64_t as, const void* y, int64_t b, int64_t bs, int64_t m) {
+  const uintptr_t px = reinterpret_cast<uintptr_t>(x), py = reinterpret_cast<uintptr_t>(y);
+  if (px + (uintptr_t)((m - 1) * as + a) <= py || py + (uintptr_t)((m - 1) * bs + b) <= px) return false;
+  for (int64_t i = 0; i < m; ++i)
+    for (int64_t j = 0; j < m; ++j) {
+      const uintptr_t u = px + (uintptr_t)(i * as), v = py + (uintptr_t)(j * bs);
+      if (u < v + (uintptr_t)b && v < u + (uintptr_t)a) return true;
+    }
+  return false;
+}
+
 #define RG_CHECK(expr)                \
   do {                                \
     const rg_status st_ = (expr);     \
@@ -145,6 +158,10 @@ rg_status rg_linear_i8_token(const rg_linear_token_args* p, void* workspace, int
   float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + round_up(p->m * p->ld, 256));
   RG_CHECK(check_rows(f, p->x, p->x_dtype, p->m, p->k, p->ldx, p->ld));
   if (p->m == 0) return RG_OK;
+  // every block of the one launch reads all of x, also after others have stored their outputs
+  const int64_t sx = dtype_size(p->x_dtype), so = dtype_size(p->out_dtype);
+  if (skinny && rows_overlap(p->x, p->k * sx, p->ldx * sx, p->out, p->n * so, p->ldo * so, p->m))
+    return refuse(RG_ERR_INVALID_ARG, "%s: x and out overlap, which this size (no workspace, one launch) cannot take", f);
   TokenGemmArgs g;
   g.a = q; g.a_scale = scale; g.w = p->w; g.w_scale = p->w_scale; g.bias = p->bias;
   g.m = p->m; g.n = p->n; g.ld = p->ld; g.ldo = p->ldo; g.act = p->act; g.act_param = p->act_param;

@@ -84,7 +84,7 @@ def linear_i8_token(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bia
     """act(x W^T + bias) with x [..., k] quantized to i8 row by row and w [n, ld], w_scale [n]
     from ``quantize_weight_i8`` (ld >= k).  The product is exact in 32-bit integers; its scale
     is row scale * channel scale; the result is rounded once to ``out_dtype`` (default: x's).
-    ``act``: an activation name or :class:`Activation`.  f32 results follow the framework's
+    ``out`` may be ``x`` or overlap it.  ``act``: an activation name or :class:`Activation`.  f32 results follow the framework's
     activations bit for bit; 16-bit GELU and SiLU are within their own rounding of them."""
     if isinstance(act, Activation):
         code, param = act.code, act.param

@@ -167,6 +167,23 @@ def test_linear_strided_rows(gpu, sv, k, xt):
     same(torch, three.view(6, 48), want)
 
 
+@pytest.mark.parametrize("m,k", [(1, 4096), (4, 2048), (8, 1024), (3, 96), (40, 512), (300, 512)])
+@pytest.mark.parametrize("xt", ["f32", "bf16"])
+def test_linear_in_place(gpu, sv, m, k, xt):
+    """out = x, and out one row further in the same memory, at every kernel's sizes."""
+    torch = gpu
+    x, wq, sw, b = linear_case(m, k, k, seed=m)
+    w, ws, bias = torch.from_numpy(wq).cuda(), torch.from_numpy(sw).cuda(), torch.from_numpy(b).cuda()
+    memory = torch.zeros((m + 1, k), dtype=dtype(torch, xt), device="cuda")
+    x = torch.from_numpy(x).to(memory.dtype)
+    want = rounded(torch, linear_reference(x.float().numpy(), wq, sw, b, 1), xt)
+    for first in (0, 1):
+        memory[:m] = x.cuda()
+        out = memory[first:first + m]
+        assert sv.linear_i8_token(memory[:m], w, ws, bias=bias, act="relu", out=out) is out
+        same(torch, out, want)
+
+
 def test_linear_wider_weight_rows(gpu, sv):
     """ld beyond k rounded up: the tail columns of x count as zeros."""
     torch = gpu

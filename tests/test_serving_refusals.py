@@ -57,6 +57,16 @@ def test_linear(change, match, ws):
     refused("rg_linear_i8_token", INVALID, match, C.byref(linear(**change)), ws, A, None)
 
 
+@pytest.mark.parametrize("change", [
+    dict(out=A), dict(out=A + 29 * 4), dict(out=A + 3 * 30 * 4 + 29 * 4), dict(x=A + 16, out=A),
+    dict(x=A + 3 * 32 + 28, out=A), dict(ldx=64, ldo=64, out=A + 26 * 4), dict(k=16, ldx=16, ld=16, x_dtype=1, out=A + 96)])
+def test_linear_in_one_launch_refuses_an_overlap(change):
+    """Few tokens run in one launch that reads x while it writes out."""
+    assert _native.lib().rg_linear_i8_token_workspace_size(4, 8, 32) == 0
+    args = linear(**change)
+    refused("rg_linear_i8_token", INVALID, "overlap", C.byref(args), None, A, None)
+
+
 def test_linear_needs_its_workspace():
     big = linear(m=300)
     for ws in (None, U):
