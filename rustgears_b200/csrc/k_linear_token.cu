@@ -210,11 +210,12 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // exponent and reciprocal (relative error below 2^-19, far under the result's own rounding):
 // 7 instructions a value instead of about 90, which would outlast the products of a
 // 4096-long reduction.
-__device__ __forceinline__ float smooth16(int32_t act, float x) {  // GELU or SiLU
-  // GELU: 0.5 x (1 + tanh u) = x / (1 + e^(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
-  const float c1 = act == ACT_GELU ? -2.0f * 0.7978846f * 1.44269504f : -1.44269504f;
-  const float c3 = act == ACT_GELU ? c1 * 0.044715f : 0.0f;
-  return x * rcp_approx(1.0f + mma16::ex2(x * fmaf(x * x, c3, c1)));
+template <bool GELU>
+__device__ __forceinline__ float smooth16(float x) {
+  // GELU: 0.5 x (1 + tanh u) = x / (1 + e^(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3).  (x x may
+  // overflow: the exponent is infinite then, of the right sign.)
+  constexpr float c1 = GELU ? -2.0f * 0.7978846f * 1.44269504f : -1.44269504f, c3 = c1 * 0.044715f;
+  return x * rcp_approx(1.0f + mma16::ex2(x * (GELU ? fmaf(x * x, c3, c1) : c1)));
 }
 
 template <typename T, int N>
@@ -225,9 +226,14 @@ __device__ __forceinline__ void activate(float (&y)[N], int32_t act, float param
     for (int j = 0; j < N; ++j) y[j] = fmaxf(y[j], 0.0f);
     return;
   }
-  if (sizeof(T) == 2 && (act == ACT_GELU || act == ACT_SILU)) {
+  if (sizeof(T) == 2 && act == ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) y[j] = smooth16(act, y[j]);
+    for (int j = 0; j < N; ++j) y[j] = smooth16<true>(y[j]);
+    return;
+  }
+  if (sizeof(T) == 2 && act == ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) y[j] = smooth16<false>(y[j]);
     return;
   }
   if (act == ACT_GELU) {
@@ -863,9 +869,9 @@ __global__ void __launch_bounds__(kSkinnyThreads, 3) k_linear_skinny(const Skinn
         for (int i = 0; i < kSkinnyWarps; ++i) sum += part[i][r][t];
         const float y = dequant(sum, __fmul_rn(scales[t], g.w_scale[n]), g.bias ? g.bias[n] : 0.0f);
         static_cast<TO*>(g.out)[t * g.ldo + n] =
-            ElemOf<TO>::from(sizeof(TO) == 2 && (g.act == ACT_GELU || g.act == ACT_SILU)
-                                 ? smooth16(g.act, y)
-                                 : act_apply(g.act, g.act_param, y));
+            ElemOf<TO>::from(sizeof(TO) == 2 && g.act == ACT_GELU   ? smooth16<true>(y)
+                             : sizeof(TO) == 2 && g.act == ACT_SILU ? smooth16<false>(y)
+                                                                    : act_apply(g.act, g.act_param, y));
       }
     }
   }

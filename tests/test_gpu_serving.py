@@ -132,6 +132,35 @@ def test_linear_activations(gpu, sv, act, code, param, m, k, n, bias):
             same(torch, got, rounded(torch, want, ot))
 
 
+def smooth_exact(act, y):
+    """GELU (tanh form, the framework's f32 constant) and SiLU of f32 values in 64 bits."""
+    y = y.astype(np.float64)
+    a = -y if act == "silu" else -2.0 * float(np.float32(0.7978846)) * (y + 0.044715 * y ** 3)
+    with np.errstate(over="ignore"):
+        return y / (1.0 + np.exp(a))
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("ot", ["f16", "bf16"])
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_linear_smooth_activations_of_large_values(gpu, sv, act, ot, m):
+    """Finite pre-activations of any size: the value itself (or the type's infinity) above, 0 below."""
+    torch = gpu
+    x, wq, _, _ = linear_case(m, 64, 48, seed=m, outlier=False)
+    # |pre-activation| of a channel about 3 * 64 * 40 times its scale
+    sw = np.logspace(-4, 34, 48).astype(np.float32)
+    pre = linear_reference(x, wq, sw, None, 0)
+    assert np.isfinite(pre).all() and pre.max() > 1e36 and pre.min() < -1e36
+    got = run_linear(torch, sv, x, wq, sw, None, act, "f32", ot).double().cpu().numpy()
+    want = smooth_exact(act, pre)
+    assert (got[pre < -120.0] == 0).all()
+    # one rounding to the type, 2^-5 of it for the f32 evaluation, the type's smallest step
+    u, step, most = (2.0 ** -11, 2.0 ** -25, 65504.0) if ot == "f16" else (2.0 ** -8, 2.0 ** -134, 3.38e38)
+    assert np.isposinf(got[want > most * (1 + 2 * u)]).all()
+    near = (pre > (-9.0 if act == "gelu" else -80.0)) & (want < most * (1 - 2 * u))
+    assert near.sum() > 10 and (np.abs(got - want)[near] <= (u * (1 + 2.0 ** -5) * np.abs(want) + step)[near]).all()
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
 def test_linear_special_rows(gpu, sv, m):
     """Rows of zeros, tiny rows, NaN and infinities touch no other row."""
