@@ -206,16 +206,21 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 
 // Activation of N pre-activation values.  f32 results follow the framework's restatements
-// bit for bit.  For 16-bit results GELU and SiLU are x / (1 + 2^(..)) on the hardware's
-// exponent and reciprocal (relative error below 2^-19, far under the result's own rounding):
-// 7 instructions a value instead of about 90, which would outlast the products of a
-// 4096-long reduction.
+// bit for bit.  For 16-bit results GELU and SiLU are x / (1 + 2^a) on the hardware's exponent
+// and reciprocal: 8 instructions a value instead of about 90, which would outlast the products
+// of a 4096-long reduction.  Relative error: 2^-20 where the result is of x's size, and with
+// the f32 rounding of a about 2^-22 |a| more where it vanishes (GELU 2^-17.4 at x = -7,
+// 2^-16 at -10; SiLU 2^-19 at -40, 2^-18 at -87), under 1/16 of the types' half steps of 2^-9 and
+// 2^-12; bf16's subnormal results are within one of their steps.
 template <bool GELU>
 __device__ __forceinline__ float smooth16(float x) {
   // GELU: 0.5 x (1 + tanh u) = x / (1 + e^(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3).  (x x may
-  // overflow: the exponent is infinite then, of the right sign.)
+  // overflow: the exponent is infinite then, of the right sign.)  Numerator and denominator are
+  // taken times 2^-14: 1 + 2^a has a normal reciprocal up to a = 126 only, but x / (1 + 2^a) is a
+  // bf16 number up to a = 140.
   constexpr float c1 = GELU ? -2.0f * 0.7978846f * 1.44269504f : -1.44269504f, c3 = c1 * 0.044715f;
-  return x * rcp_approx(1.0f + mma16::ex2(x * (GELU ? fmaf(x * x, c3, c1) : c1)));
+  const float a = fmaf(x, GELU ? fmaf(x * x, c3, c1) : c1, -14.0f);
+  return (x * 0x1p-14f) * rcp_approx(0x1p-14f + mma16::ex2(a));
 }
 
 template <typename T, int N>

@@ -161,6 +161,21 @@ def test_linear_smooth_activations_of_large_values(gpu, sv, act, ot, m):
     assert near.sum() > 10 and (np.abs(got - want)[near] <= (u * (1 + 2.0 ** -5) * np.abs(want) + step)[near]).all()
 
 
+@pytest.mark.parametrize("act,lowest", [("gelu", -12.0), ("silu", -110.0)])
+@pytest.mark.parametrize("ot", ["f16", "bf16"])
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_linear_smooth_activations_vanish_late(gpu, sv, act, lowest, ot, m):
+    """The negative tails, down to the type's smallest numbers: rows of zeros leave the bias."""
+    torch = gpu
+    pre = np.concatenate([np.linspace(lowest, 1.0, 3000), -np.logspace(-44, 0, 500)]).astype(np.float32)
+    x, wq, sw, _ = linear_case(m, 32, len(pre), seed=m, outlier=False)
+    got = run_linear(torch, sv, x * 0, wq, sw, pre, act, "f32", ot).double().cpu().numpy()
+    want = smooth_exact(act, pre)[None, :]
+    # one rounding to the type, 2^-5 of it for the f32 evaluation; the type's smallest step
+    u, step = (2.0 ** -11, 2.0 ** -24) if ot == "f16" else (2.0 ** -8, 2.0 ** -133)
+    assert (np.abs(got - want) <= u * (1 + 2.0 ** -5) * np.abs(want) + step).all()
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
 def test_linear_special_rows(gpu, sv, m):
     """Rows of zeros, tiny rows, NaN and infinities touch no other row."""
