@@ -449,7 +449,9 @@ rg_status rg_kv_append(const rg_kv_cache* cache, const rg_kv_append_args* args, 
  * key being zeros.  q and out have the cache's dtype; scores, the softmax's maximum and sum,
  * and the output sum are f32; a probability is rounded to the cache's dtype before it
  * multiplies v.  max_q_len and max_kv_len bound the lengths (they size the launch); a
- * sequence whose lengths are out of range is reported and skipped.  head_dim: 64, 96, 128 or
+ * sequence whose lengths are out of range is reported and skipped.  out is written for the
+ * tokens of the other sequences only: rows that no cu_q range names (padding) and those of a
+ * skipped sequence keep what they held.  head_dim: 64, 96, 128 or
  * 256.  `workspace`: rg_attention_paged_workspace_size bytes, 256-byte aligned (NULL when
  * that is 0), free again once the call's work on `stream` is done. */
 typedef struct rg_paged_attention_args {

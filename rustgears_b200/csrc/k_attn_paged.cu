@@ -400,7 +400,7 @@ rg_status go(const AttnParams& A, cudaStream_t st) {
   const auto kernel = k_attn_few<T, D, WR, WK>;
   static DeviceOnce once;
   once.run([&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); });
-  const int64_t rows = std::min<int64_t>((int64_t)A.p.a.max_q_len * A.group.d, A.max_rows);
+  const int64_t rows = std::min<int64_t>((int64_t)std::max(A.p.a.max_q_len, 1) * A.group.d, A.max_rows);
   const int64_t tiles = (rows + S::kRows - 1) / S::kRows;
   if (tiles * A.splits > INT_MAX) return RG_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)(tiles * A.splits), (unsigned)A.p.c.kv_heads, (unsigned)A.p.a.batch);
@@ -502,11 +502,12 @@ rg_status make_plan(const PagedAttnArgs& p, Plan& L) {
   A.splits = 1;
   A.part_o = nullptr;
   A.part_ml = nullptr;
-  L.rows = (int64_t)p.a.max_q_len * A.group.d;
+  // (max_q_len 0: one block per sequence and head reports those that have tokens)
+  L.rows = (int64_t)std::max(p.a.max_q_len, 1) * A.group.d;
   if (L.rows > INT_MAX || p.c.kv_heads > 65535) return RG_ERR_UNSUPPORTED;
   // Chunks go to the tensor-core kernel.  Where the batch may hold shorter sequences too (the
   // tokens are fewer than batch times the longest), those take the kernel for few rows.
-  L.many = L.rows > kFewRows && attention_tc_takes(p);
+  L.many = p.a.max_q_len > 0 && L.rows > kFewRows && attention_tc_takes(p);
   L.few = !L.many || (p.a.batch > 1 && p.a.tokens < (int64_t)p.a.batch * p.a.max_q_len);
   A.min_rows = 0;
   A.max_rows = L.many ? kFewRowsBeside : INT_MAX;
@@ -515,7 +516,7 @@ rg_status make_plan(const PagedAttnArgs& p, Plan& L) {
   const int64_t seqs = (int64_t)p.c.kv_heads * p.a.batch;
   L.few_shape = {few_rows(A), few_keys(d), 1};
   L.many_shape = {kTcRows, kTcKeys, 1};
-  if (L.few) {
+  if (L.few && p.a.max_q_len > 0) {
     // (beside chunks: taken as one block for every other sequence)
     const int64_t blocks = L.many ? (seqs + 1) / 2 : seqs * ((L.rows + L.few_shape.rows - 1) / L.few_shape.rows);
     // blocks an SM holds at once (Shape::kSmem)

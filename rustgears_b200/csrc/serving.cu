@@ -288,7 +288,7 @@ rg_status rg_attention_paged(const rg_kv_cache* cache, const rg_paged_attention_
                              int32_t* error_words, void* stream) {
   const char* f = "rg_attention_paged";
   RG_CHECK(check_attention(f, cache, args));
-  if (args->batch == 0 || args->tokens == 0 || args->max_q_len == 0) return RG_OK;
+  if (args->batch == 0 || args->tokens == 0) return RG_OK;  // (max_q_len 0: the lengths are looked at all the same)
   if (!args->q || !args->out || !args->kv_len || !args->cu_q || !error_words ||
       (!args->block_table && args->max_kv_len > 0))
     return refuse(RG_ERR_INVALID_ARG, "%s: null argument", f);

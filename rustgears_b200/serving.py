@@ -147,7 +147,11 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     all int32).  ``causal``: its tokens are the last of its keys, each seeing itself and what
     is before it.  A row that sees no key is zeros.  heads is a multiple of the cache's heads
     (shared in order); head_dim 64, 96, 128 or 256.  ``max_q_len`` and ``max_kv_len`` (default:
-    what the table can hold) bound the lengths; ``scale`` defaults to 1 / sqrt(head_dim)."""
+    what the table can hold) bound the lengths: a sequence beyond them is reported by
+    :func:`check` and skipped.  Rows of the result that no sequence owns (padding behind
+    ``cu_q[-1]``), and a skipped sequence's, are not written: they keep what ``out`` held, or
+    hold anything when the result is allocated here.  ``scale`` defaults to
+    1 / sqrt(head_dim)."""
     return _bind.attention(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q_len, max_kv_len, scale, causal, out)
 
 

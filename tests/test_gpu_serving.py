@@ -670,6 +670,36 @@ def test_attention_reports_lengths_and_pages_out_of_range(gpu, sv):
         assert (out[most:2 * most] == 3).all()
 
 
+@pytest.mark.parametrize("dim,heads", [(64, 4), (128, 160)])
+def test_attention_without_tokens_by_its_bound(gpu, sv, dim, heads):
+    """max_q_len 0 is a bound like any other: sequences that have tokens are reported, empty ones
+    (all rows padding) are not; no row is written."""
+    torch = gpu
+    q, kc, vc, table, kv_len, cu = make_batch(torch, [(3, 40), (2, 9)], heads, 2, dim, torch.bfloat16, 16, "token")
+    out = torch.full_like(q, 3.0)
+    sv.attention_paged(q, kc, vc, table, kv_len, cu, max_q_len=0, max_kv_len=40, out=out)
+    with pytest.raises(_native.RgError, match="length"):
+        sv.check()
+    sv.attention_paged(q, kc, vc, table, kv_len, cu * 0, max_q_len=0, max_kv_len=40, out=out)
+    sv.check()
+    assert (out == 3).all()
+
+
+def test_attention_leaves_rows_of_no_sequence_alone(gpu, sv):
+    """Padding before and behind the sequences' tokens is not written."""
+    torch = gpu
+    for most in (1, 150):
+        lens = [(most, 200), (most, 170)]
+        q, kc, vc, table, kv_len, cu = make_batch(torch, lens, 4, 2, 64, torch.float16, 16, "token", seed=4)
+        want = sv.attention_paged(q, kc, vc, table, kv_len, cu, max_q_len=most, max_kv_len=200)
+        wide = torch.full((q.shape[0] + 7, 4, 64), 5.0, dtype=q.dtype, device="cuda")
+        wide[2:2 + 2 * most] = q
+        out = torch.full_like(wide, 3.0)
+        sv.attention_paged(wide, kc, vc, table, kv_len, cu + 2, max_q_len=most, max_kv_len=200, out=out)
+        same(torch, out[2:2 + 2 * most], want)
+        assert (out[:2] == 3).all() and (out[2 + 2 * most:] == 3).all()
+
+
 def test_attention_cache_beyond_32_bit_offsets(gpu, sv):
     """Pages whose element offset exceeds 2^32 (the same tensor serves as keys and values)."""
     torch = gpu
