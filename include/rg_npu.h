@@ -346,12 +346,18 @@ rg_status rg_selftest_fast_paths(uint64_t mismatches[6]);
  * host, so they can be captured.  What only the device can see (a bounded wait
  * that gave up, a position, slot, page or length out of its range) is reported
  * through `error_words`: two zeroed int32 words of device memory that any number
- * of calls may share; a call only ever sets them, and
- * rg_status_from_error_words maps a host copy to a status.  What an out-of-range
+ * of calls may share; a call only ever sets them.  rg_take_error_words moves them out,
+ * and rg_status_from_error_words maps a host copy to a status.  What an out-of-range
  * index names is never accessed: the token, page or sequence is skipped (its
  * output is not written, or a page's keys count as zeros).
  * A call of zero rows, tokens or sequences returns RG_OK and launches nothing.
  * ------------------------------------------------------------------------- */
+/* Moves the two error words to `taken` (device memory, two int32) and zeroes them in one
+ * atomic step each, in the order of `stream`: what calls on other streams or threads set
+ * meanwhile is either in `taken` or still in the words, never lost (copying and then
+ * zeroing them loses it). */
+rg_status rg_take_error_words(int32_t* error_words, int32_t* taken, void* stream);
+
 typedef enum rg_dtype { RG_DTYPE_F32 = 0, RG_DTYPE_F16 = 1, RG_DTYPE_BF16 = 2 } rg_dtype;
 
 /* One scale per row (token): x [rows, k] (row stride ldx elements) -> q [rows, ldq] i8

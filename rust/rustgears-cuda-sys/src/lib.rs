@@ -343,6 +343,7 @@ extern "C" {
                                 bias: *const f32, act: i32, act_param: f32, out: *mut f32,
                                 stream: *mut c_void) -> rg_status;
     pub fn rg_status_from_error_words(words: *const i32) -> rg_status;
+    pub fn rg_take_error_words(error_words: *mut i32, taken: *mut i32, stream: *mut c_void) -> rg_status;
     pub fn rg_debug_set_tc_wait(wait_ns: u64, starve_loads: i32);
     pub fn rg_maxpool2d_f32(x: *const f32, n: i64, c: i32, h: i32, w: i32, k: i32, stride: i32, y: *mut f32,
                             stream: *mut c_void) -> rg_status;

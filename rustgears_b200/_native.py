@@ -158,6 +158,7 @@ SIGNATURES = {
     "rg_attention_f32": ([_vp, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _vp], _i32),
     "rg_activation_f32": ([_vp, _i64, _i32, _f32, _vp, _vp], _i32),
     "rg_selftest_fast_paths": ([_vp], _i32),
+    "rg_take_error_words": ([_vp, _vp, _vp], _i32),
     "rg_quantize_token_i8": ([_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp], _i32),
     "rg_gemm_i8_token": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _f32, _vp, _i32, _i64, _vp, _vp], _i32),
     "rg_linear_i8_token_workspace_size": ([_i64, _i64, _i64], _i64),

@@ -86,6 +86,8 @@ bool rows_overlap(const void* x, int64_t a, int64_t as, const void* y, int64_t b
     if (st_ != RG_OK) return st_;     \
   } while (0)
 
+__global__ void k_take_words(int32_t* words, int32_t* taken) { taken[threadIdx.x] = atomicExch(words + threadIdx.x, 0); }
+
 rg_status check_cache(const char* f, const rg_kv_cache* c) {
   if (!c) return refuse(RG_ERR_INVALID_ARG, "%s: null cache", f);
   if (c->dtype != RG_DTYPE_F16 && c->dtype != RG_DTYPE_BF16)
@@ -112,6 +114,14 @@ rg_status check_rotation(const char* f, const int32_t* positions, const float* t
 }  // namespace
 
 extern "C" {
+
+rg_status rg_take_error_words(int32_t* error_words, int32_t* taken, void* stream) {
+  const char* f = "rg_take_error_words";
+  if (!error_words || !taken) return refuse(RG_ERR_INVALID_ARG, "%s: null argument", f);
+  if (!aligned(error_words, 4) || !aligned(taken, 4)) return refuse(RG_ERR_INVALID_ARG, "%s: misaligned words", f);
+  k_take_words<<<1, 2, 0, (cudaStream_t)stream>>>(error_words, taken);
+  return launched(f, RG_OK);
+}
 
 rg_status rg_quantize_token_i8(const void* x, int32_t x_dtype, int64_t rows, int64_t k, int64_t ldx, int8_t* q,
                                int64_t ldq, float* scale, void* stream) {

@@ -48,7 +48,8 @@ _SCALING = {"plain": _native.RG_ROPE_PLAIN, "linear": _native.RG_ROPE_LINEAR, "b
 
 def check(device: int | torch.device | str | None = None) -> None:
     """Waits for ``device`` (default: the current one) and raises what its serving calls
-    reported since the last check (``RgError``), clearing it."""
+    reported since the last check (``RgError``), clearing it.  The report is the device's: it
+    covers the calls of every thread and stream, and one check takes it for all of them."""
     if device is None:
         device = torch.cuda.current_device()
     elif not isinstance(device, int):
@@ -58,10 +59,12 @@ def check(device: int | torch.device | str | None = None) -> None:
     if words is None:
         return
     torch.cuda.synchronize(device)
-    host = words.tolist()
+    with torch.cuda.device(device):
+        taken = torch.empty_like(words)
+        _native.check(_native.lib().rg_take_error_words(words.data_ptr(), taken.data_ptr(),
+                                                        torch.cuda.current_stream().cuda_stream))
+        host = taken.tolist()
     if host != [0, 0]:
-        words.zero_()
-        torch.cuda.synchronize(device)
         _native.check(_native.lib().rg_status_from_error_words((C.c_int32 * 2)(*host)))
 
 

@@ -865,6 +865,28 @@ def test_attention_long_chunks(gpu, sv, dim, page):
                         seed=page)
 
 
+def test_check_loses_no_report(gpu, sv, monkeypatch):
+    """What another caller's kernel reports while a check is under way is raised by the next one."""
+    torch = gpu
+    table = sv.rope_table(4, 64)
+    x, far = torch.zeros(1, 1, 64, device="cuda"), torch.tensor([99], dtype=torch.int32, device="cuda")
+    read = torch.Tensor.tolist
+
+    def read_then_report(t):
+        host = read(t)
+        monkeypatch.setattr(torch.Tensor, "tolist", read)
+        sv.rope(x, far, table)
+        torch.cuda.synchronize()
+        return host
+
+    sv.rope(x, far, table)
+    monkeypatch.setattr(torch.Tensor, "tolist", read_then_report)
+    for _ in range(2):
+        with pytest.raises(_native.RgError, match="position"):
+            sv.check()
+    sv.check()
+
+
 def test_zero_sizes(gpu, sv):
     torch = gpu
     w, ws = sv.quantize_weight_i8(torch.randn(8, 32, device="cuda"))

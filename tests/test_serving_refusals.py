@@ -115,6 +115,11 @@ def test_rope_needs_error_words():
     refused("rg_rope", INVALID, "null", None, A, None)
 
 
+@pytest.mark.parametrize("words,taken,match", [(None, A, "null"), (A, None, "null"), (A + 2, A, "misaligned")])
+def test_take_error_words(words, taken, match):
+    refused("rg_take_error_words", INVALID, match, words, taken, None)
+
+
 def cache(**change):
     return _native.KvCacheC(**{**dict(k=A, v=A, dtype=1, page_size=16, kv_heads=2, head_dim=64, pages=10,
                                       page_stride=2048, token_stride=128, head_stride=64), **change})
