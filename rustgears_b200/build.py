@@ -1,5 +1,5 @@
 """Builds librg_npu.so (all CUDA kernels + the C ABI) in-tree for sm_100a, and the binding of
-its serving entry points to torch tensors (_serving_bind.so)."""
+its serving entry points to torch tensors (_serving_bind.so) where a CUDA torch is installed."""
 from __future__ import annotations
 
 import glob
@@ -53,20 +53,23 @@ def _compile(src: str) -> str:
     return obj
 
 
-def _torch_dir() -> str:
+def _torch_dir() -> str | None:
+    """The installed torch's folder; None where there is none, or one without CUDA."""
     import importlib.util
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
-        raise RuntimeError("torch not found")
-    return list(spec.submodule_search_locations)[0]
+        return None
+    torch = list(spec.submodule_search_locations)[0]
+    return torch if os.path.exists(os.path.join(torch, "lib", "libtorch_cuda.so")) else None
 
 
-def build_binding() -> str:
-    """Compiles bind/serving_bind.cpp against torch's headers and links it to librg_npu.so."""
-    header = os.path.join(ROOT, "include", "rg_npu.h")
-    if os.path.exists(BIND) and os.path.getmtime(BIND) >= max(os.path.getmtime(f) for f in (BIND_SRC, header)):
-        return BIND
+def build_binding() -> str | None:
+    """Compiles bind/serving_bind.cpp against torch's headers and links it to librg_npu.so.
+    None without a CUDA torch: the library (C ABI, Rust crate, sessions) needs none, only
+    rustgears_b200.serving does."""
     torch = _torch_dir()
+    if torch is None:
+        return None
     cuda = os.path.dirname(os.path.dirname(NVCC))
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
            "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
@@ -74,6 +77,9 @@ def build_binding() -> str:
            "-I", os.path.join(cuda, "include"), BIND_SRC, "-o", BIND,
            "-L", os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
            "-L", HERE, "-l:librg_npu.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(torch, "lib")]
+    header = os.path.join(ROOT, "include", "rg_npu.h")
+    if os.path.exists(BIND) and os.path.getmtime(BIND) >= max(os.path.getmtime(f) for f in (BIND_SRC, header)):
+        return BIND
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {BIND} failed:\n{r.stdout}\n{r.stderr}")
@@ -94,9 +100,11 @@ def build(verbose: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    build_binding()
+    bound = build_binding()
     if verbose:
         print("built", LIB)
+        if bound is None:
+            print("no CUDA torch: rustgears_b200.serving has no binding")
     return LIB
 
 
