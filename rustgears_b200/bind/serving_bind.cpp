@@ -507,4 +507,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving_bind", nullptr, -1, metho
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__serving_bind() { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__serving_bind() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", RG_TORCH_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import glob
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -64,25 +65,34 @@ def _torch_dir() -> str | None:
 
 
 def build_binding() -> str | None:
-    """Compiles bind/serving_bind.cpp against torch's headers and links it to librg_npu.so.
-    None without a CUDA torch: the library (C ABI, Rust crate, sessions) needs none, only
-    rustgears_b200.serving does."""
+    """Compiles bind/serving_bind.cpp against torch's headers and links it to librg_npu.so, again
+    when its source, the C header, torch or Python changed.  None without a CUDA torch: the
+    library (C ABI, Rust crate, sessions) needs none, only rustgears_b200.serving does."""
     torch = _torch_dir()
     if torch is None:
         return None
+    with open(os.path.join(torch, "version.py")) as f:
+        text = f.read()
+    version = re.search(r"""^__version__\s*=\s*['"]([^'"]+)""", text, flags=re.M)
     cuda = os.path.dirname(os.path.dirname(NVCC))
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           f'-DRG_TORCH_VERSION="{version.group(1) if version else "unknown"}"',
            "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
            "-I", os.path.join(torch, "include"), "-I", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
            "-I", os.path.join(cuda, "include"), BIND_SRC, "-o", BIND,
            "-L", os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
            "-L", HERE, "-l:librg_npu.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(torch, "lib")]
-    header = os.path.join(ROOT, "include", "rg_npu.h")
-    if os.path.exists(BIND) and os.path.getmtime(BIND) >= max(os.path.getmtime(f) for f in (BIND_SRC, header)):
+    built_for = "\n".join([sysconfig.get_config_var("SOABI") or sys.version, text] + cmd)
+    header, key = os.path.join(ROOT, "include", "rg_npu.h"), os.path.join(OBJ, os.path.basename(BIND) + ".built_for")
+    if os.path.exists(BIND) and os.path.getmtime(BIND) >= max(os.path.getmtime(f) for f in (BIND_SRC, header)) and \
+            os.path.exists(key) and open(key).read() == built_for:
         return BIND
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {BIND} failed:\n{r.stdout}\n{r.stderr}")
+    os.makedirs(OBJ, exist_ok=True)
+    with open(key, "w") as f:
+        f.write(built_for)
     return BIND
 
 

@@ -39,6 +39,9 @@ try:
     from . import _serving_bind as _bind
 except ImportError as e:
     raise ImportError(f"{e}: build it with `python -m rustgears_b200.build` (a CUDA torch is needed)") from e
+if _bind.torch_version != torch.__version__:
+    raise ImportError(f"_serving_bind was built for torch {_bind.torch_version}, this is {torch.__version__}: build it "
+                      "again with `python -m rustgears_b200.build`")
 _bind.set_check(_native.check)
 
 _ACT = {"none": (0, 0.0), "relu": (1, 0.0), "sigmoid": (2, 0.0), "tanh": (3, 0.0), "gelu": (4, 0.0),

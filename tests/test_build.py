@@ -1,6 +1,7 @@
-"""What the build needs."""
+"""What the build needs and when it builds the torch binding again."""
 import importlib.util
 import os
+import sysconfig
 import types
 
 import pytest
@@ -41,7 +42,33 @@ def fake_torch(monkeypatch, tmp_path):
     return torch, runs
 
 
+def test_binding_follows_torch_and_python(fake_torch, monkeypatch):
+    torch, runs = fake_torch
+    for _ in range(2):
+        assert build.build_binding() == build.BIND
+    assert len(runs) == 1
+    (torch / "version.py").write_text("__version__ = '9.9.2+cu1'\n")
+    build.build_binding()
+    build.build_binding()
+    assert len(runs) == 2 and any("9.9.2+cu1" in a for a in runs[1])
+    var = sysconfig.get_config_var
+    monkeypatch.setattr(sysconfig, "get_config_var", lambda name: "cpython-399" if name == "SOABI" else var(name))
+    build.build_binding()
+    build.build_binding()
+    assert len(runs) == 3
+
+
 def test_no_binding_for_a_torch_without_cuda(fake_torch):
     torch, runs = fake_torch
     (torch / "lib" / "libtorch_cuda.so").unlink()
     assert build.build_binding() is None and not runs
+
+
+def test_binding_names_its_torch(monkeypatch):
+    torch = pytest.importorskip("torch")
+    from rustgears_b200 import serving
+    assert serving._bind.torch_version == torch.__version__
+    monkeypatch.setattr(torch, "__version__", "0.0")
+    spec = importlib.util.spec_from_file_location("rustgears_b200._serving_again", serving.__file__)
+    with pytest.raises(ImportError, match="built for torch"):
+        spec.loader.exec_module(importlib.util.module_from_spec(spec))
