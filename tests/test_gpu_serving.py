@@ -633,6 +633,24 @@ def test_attention_strided_q_and_out(gpu, sv):
         same(torch, out.contiguous(), want)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("lens", [[(1, 900), (1, 333)], [(200, 700), (1, 450)], [(300, 1000)]])
+def test_attention_cache_of_other_strides(gpu, sv, dim, lens):
+    """Caches that are views: padded heads, tokens and pages; keys and values of one page side by side."""
+    torch = gpu
+    q, kc, vc, table, kv_len, cu = make_batch(torch, lens, 6, 3, dim, torch.bfloat16, 16, "token", seed=8)
+    most = dict(max_q_len=max(a for a, _ in lens), max_kv_len=max(b for _, b in lens))
+    want = sv.attention_paged(q, kc, vc, table, kv_len, cu, **most)
+    n = kc.shape[0]
+    kp, vp = (torch.full((n, 19, 4, dim + 8), float("nan"), dtype=q.dtype, device="cuda")[:, 2:18, :3, :dim] for _ in range(2))
+    both = torch.full((n, 2, 16, 3, dim), float("nan"), dtype=q.dtype, device="cuda")
+    turned = torch.full((3, n, 2, 16, dim), float("nan"), dtype=q.dtype, device="cuda")
+    for k, v in ((kp, vp), (both[:, 0], both[:, 1]), (turned[:, :, 0].permute(1, 2, 0, 3), turned[:, :, 1].permute(1, 2, 0, 3))):
+        k.copy_(kc)
+        v.copy_(vc)
+        same(torch, sv.attention_paged(q, k, v, table, kv_len, cu, **most), want)
+
+
 def test_attention_repeats_bit_for_bit(gpu, sv):
     torch = gpu
     for lens in ([(1, 5000)], [(300, 900), (1, 2000), (77, 77)]):
