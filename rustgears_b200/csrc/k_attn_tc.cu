@@ -4,7 +4,8 @@
 // A block takes 256 rows (two groups of 128) of one (sequence, key head), row r = token
 // r / group, head r % group, and walks the sequence's keys in tiles of 128:
 //   S_g = Q_g K^T   tcgen05, both operands in shared memory, S in TMEM (128 columns a group)
-//   P_g = 2^(S_g scale2 - m), rounded to the cache's type, written over S_g in TMEM
+//   P_g = 2^(S_g scale2 - m), rounded to the cache's type (both operands of a product have
+//                   one type; the row sum adds P unrounded), written over S_g in TMEM
 //   O_g += P_g V    tcgen05, P from TMEM, V from shared memory as it was loaded (keys are the
 //                   product's K dimension: V is the "transposed" operand), O in TMEM
 // One thread per row does the softmax, so a row's maximum and sum need no exchange; its 128
@@ -19,7 +20,8 @@
 // are full at once at best, 2048 clocks for both groups.  Measured 3300: a group's chain of load
 // (95 clocks), maximum (320), exponentials (1430), store and arrival (150), then its products, is
 // longer than twice the tensor time.  2048 new tokens over 16384 keys, 32 query heads on 8 of 128:
-// 479 us = 1076 TFLOP/s (256 blocks on 148 SMs: two rounds where 1.73 have work).  Every fourth
+// 478 to 509 us from run to run, 1077 to 1013 TFLOP/s (the power cap; 256 blocks on 148 SMs: two
+// rounds where 1.73 have work).  Every fourth
 // pair of exponentials as a polynomial on the FMA pipes: 545 us, not kept.
 //   warp 0     TMA: a page's part of a tile is one box per 64 dimensions (page sizes that
 //              divide 128 or are multiples of it), so a tile arrives swizzled whatever its pages

@@ -167,7 +167,8 @@ void quantize(const void* x, int64_t rows, int64_t k, int64_t ldx, int8_t* q, in
 // 96 bytes a clock in and 96 out, of 128).  For few rows it is the stream of W: rows of A past
 // m are filled with zeros without traffic, and narrow tiles spread W over all SMs.
 // Measured alone: 16384 x 8192 x 8192 660 us = 3330 TOPS, 4096 x 8192 x 8192 163 us = 3380 (tensor
-// pipe 91 % active); 2048 x 4096 x 14336 + GELU to f16 about 88 us.
+// pipe 91 % active); 2048 x 4096 x 14336 + GELU to f16 about 88 us (448 tiles on 74 pairs: seven
+// rounds where 6.05 have work).
 //   warp 0      TMA producer of its own CTA's operands, completing on the even CTA's barrier
 //   warp 1      of the even CTA: issues the products for both
 //   warps 2-9   epilogue: scale, bias, activation, rounding, a 64-byte-wide tile staged in
@@ -1007,7 +1008,9 @@ rg_status go_few(const TokenGemmArgs& a, cudaStream_t st) {
 template <typename T>
 rg_status go_gemm(const TokenGemmArgs& a, cudaStream_t st) {
   // Few tokens against pairs, us: 10.1 / 15.7 at 17 x 4096 x 4096, 12.5 / 16.0 at 64, 14.6 / 17.3 at 128;
-  // 18.6 / 20.8 at 64 x 4096 x 14336, 24.6 / 22.2 at 128; 10.3 / 8.1 at 128 x 1024 x 1024.
+  // 18.6 / 20.8 at 64 x 4096 x 14336, 24.6 / 22.2 at 128; 10.3 / 8.1 at 128 x 1024 x 1024.  One limit
+  // for all widths: above it wide and short layers gain, layers like 4096 x 4096 lose (11.9 us at 96
+  // tokens, 16.5 at 97).
   if (a.m <= 96) return go_few<T>(a, st);
   const auto cost = [&](int64_t bn) { return ((a.m + 255) / 256 * ((a.n + bn - 1) / bn) + 73) / 74 * (bn + 96); };
   if (cost(256) <= cost(128) && cost(256) <= cost(64)) return go_pair<256, T>(a, st);
