@@ -73,7 +73,9 @@ struct TcParams {
   uint64_t wait_ns;
   int32_t starve;
   // The launch before is the kernel for few rows, which this one does not depend on: it waits
-  // for it at its end only.  (That kernel started after whatever ran before the call was over.)
+  // for it at its end only.  (That kernel's blocks waited until whatever ran before the call was
+  // over, and this launch starts when all of them have come further.  This one has not waited
+  // itself, so nothing it reads comes through L1, which might be older: TMA, and __ldcg.)
   int32_t beside;
 };
 
@@ -133,8 +135,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!p.beside) grid_dependency_wait();
   grid_launch_dependents();
 
-  const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
-  const int kv = a.kv_len[b];
+  const int64_t q0 = __ldcg(a.cu_q + b), q1 = __ldcg(a.cu_q + b + 1);
+  const int kv = __ldcg(a.kv_len + b);
   if (q0 < 0 || q1 < q0 || q1 > a.tokens || q1 - q0 > a.max_q_len || kv < 0 || kv > a.max_kv_len) {
     if (threadIdx.x == 0) p.P.p.err[1] = 1;
     grid_dependency_wait();
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane >= per_tile || n >= tiles) return 0;
       const int key = (t0 + n) * kTile + lane * p.box;
       if (key >= kv) return 0;
-      const int page = table[p.P.page.div((uint32_t)key)];
+      const int page = __ldcg(table + p.P.page.div((uint32_t)key));
       if (page >= 0 && page < c.pages) return page;
       p.P.p.err[1] = 1;
       return (int)c.pages;  // past the last page: the copy fills zeros
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int ch = 0; ch < D / 8; ++ch) {
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (real) w = reinterpret_cast<const uint4*>(src)[ch];
+        if (real) w = __ldcg(reinterpret_cast<const uint4*>(src) + ch);
         w.x ^= p.flip; w.y ^= p.flip; w.z ^= p.flip; w.w ^= p.flip;
         *reinterpret_cast<uint4*>(dst + (ch >> 3) * C::kSub + (((ch & 7) ^ (tr & 7)) << 4)) = w;
       }

@@ -305,6 +305,52 @@ def test_calls_see_what_ran_just_before(gpu, sv):
         same(torch, copy, want[i])
 
 
+def test_mixed_batches_see_what_ran_just_before(gpu, sv):
+    """Chunks beside decoding sequences: queries, keys, lengths and pages written right before the
+    call, by an early launch and by copies, with other values in the same memory each time."""
+    torch = gpu
+    lens = [[(200, 640), (1, 600), (40, 90), (1, 33)], [(90, 500), (1, 610), (150, 150), (1, 7)]]
+    heads, hk, d, page = 4, 2, 64, 16
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n = max(sum(q for q, _ in ls) for ls in lens)
+    batches = [make_batch(torch, ls, heads, hk, d, torch.float16, page, "token", seed=i) for i, ls in enumerate(lens)]
+    pages, width = max(b[1].shape[0] for b in batches), max(b[3].shape[1] for b in batches)
+    kc, vc = (torch.zeros(pages, page, hk, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    q_out = torch.zeros(n, heads, d, dtype=torch.float16, device="cuda")
+    bt = torch.zeros(4, width, dtype=torch.int32, device="cuda")
+    kv_len, cu = (torch.zeros(k, dtype=torch.int32, device="cuda") for k in (4, 5))
+    big = torch.zeros(1 << 26, device="cuda")
+    table = sv.rope_table(8, d)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda") % 8
+    none = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    raw = torch.randn(2, n, heads, d, device="cuda", generator=g)
+    kv = torch.zeros(n, hk, d, device="cuda")
+
+    def step(i):
+        _, k, v, t, length, first = batches[i]
+        kc[:k.shape[0]] = k
+        vc[:v.shape[0]] = v
+        bt[:, :t.shape[1]] = t
+        kv_len.copy_(length)
+        cu.copy_(first)
+        sv.kv_append(kv, kv, kc, vc, none, positions=pos, table=table, q=raw[i], q_out=q_out)
+        return sv.attention_paged(q_out, kc, vc, bt, kv_len, cu, max_q_len=200, max_kv_len=640)
+
+    used = [sum(q for q, _ in ls) for ls in lens]
+    want = []
+    for i in range(2):
+        torch.cuda.synchronize()
+        want.append(step(i)[:used[i]].clone())
+        torch.cuda.synchronize()
+    got = []
+    for r in range(12):
+        if r % 4 == 0:
+            big.add_(1.0)         # long enough that the launches behind it queue up
+        got.append(step(r % 2))
+    for r, o in enumerate(got):
+        same(torch, o[:used[r % 2]], want[r % 2])
+
+
 def test_linear_kernel_level_calls(gpu, sv):
     """Quantizer and product called apart, the output a column block of a wider tensor."""
     torch, L = gpu, _native.lib()
