@@ -308,10 +308,10 @@ rg_status rg_status_from_error_words(const int32_t words[2]);
  * tcgen05 GEMM launches that follow bound every pipeline wait by wait_ns
  * (0 restores the 2 s default), and with starve_loads != 0 issue no operand
  * loads, so the first wait on them runs out and the call reports
- * RG_ERR_TIMEOUT.  starve_loads 2 is for rg_linear_i8_token of 9 to 96 tokens
- * and the chunks of rg_attention_paged (others run as with 0): the loads are
- * issued, but the products are given up before their first wait, with copies on
- * their way.  Launch parameters are fixed when a session captures its
+ * RG_ERR_TIMEOUT.  starve_loads 2 is for rg_gemm_i8_token of up to 96 tokens
+ * (also as part of rg_linear_i8_token) and the chunks of rg_attention_paged
+ * (others run as with 0): the loads are issued, but the products are given up
+ * before their first wait, with copies on their way.  Launch parameters are fixed when a session captures its
  * CUDA graph: test on host-buffer runs or RG_SESSION_NO_GRAPH sessions. */
 void rg_debug_set_tc_wait(uint64_t wait_ns, int32_t starve_loads);
 /* max_pool2d (src/kernels.rs:165-213), NCHW f32, no padding. */
